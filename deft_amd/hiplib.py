@@ -45,6 +45,20 @@ class PairMlpDesc(C.Structure):
                 ("Tper", C.c_int), ("u0", C.c_int), ("du", C.c_int), ("v0", C.c_int), ("dv", C.c_int)]
 
 
+class RotaryDesc(C.Structure):
+    """Mirror of DeftRotary (include/deft_hip.h)."""
+    _fields_ = [(n, c_fp) for n in ("q", "k", "v", "q_out", "k_out", "v_out", "pos", "freq", "axis", "q_weight", "k_weight", "row")] + \
+               [(n, C.c_longlong) for n in ("ldq", "hsq", "ldk", "hsk", "ldv", "hsv", "ldqo", "hsqo", "ldko", "hsko", "ldvo", "hsvo", "rows")] + \
+               [(n, C.c_int) for n in ("T", "Hq", "Hk", "D", "R", "A", "dtype", "pos_float", "adjacent", "inverse", "norm")] + [("eps", C.c_float)]
+
+
+class AttnDesc(C.Structure):
+    """Mirror of DeftAttn (include/deft_hip.h)."""
+    _fields_ = [(n, c_fp) for n in ("q", "k", "v", "o", "lse", "q_start", "k_start", "k_len", "ws")] + \
+               [(n, C.c_longlong) for n in ("ws_floats", "ldq", "hsq", "ldk", "hsk", "ldv", "hsv", "ldo", "hso", "ssk", "ssv")] + \
+               [(n, C.c_int) for n in ("Tq", "B", "slots", "cap", "Hq", "Hk", "D", "dtype", "causal", "max_k")] + [("scale", C.c_float)]
+
+
 _SIGS = {
     "deft_version": (C.c_int, []),
     "deft_pieces": (C.c_int, []),
@@ -81,6 +95,9 @@ _SIGS = {
     "deft_conv_direct": (C.c_int, [C.POINTER(GemmDesc), c_fp]),
     "deft_split_weights_direct": (C.c_int, [c_fp, c_fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, c_fp]),
     "deft_direct_weight_bytes": (C.c_longlong, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "deft_rotary": (C.c_int, [C.POINTER(RotaryDesc), c_fp]),
+    "deft_attn": (C.c_int, [C.POINTER(AttnDesc), c_fp]),
+    "deft_attn_ws_floats": (C.c_longlong, [C.POINTER(AttnDesc)]),
     "deft_track_similarity": (C.c_int, [c_fp] + [C.c_int] * 2 + [c_fp] * 3 + [C.c_int] * 2 + [c_fp, c_fp]),
     # host-side association helpers (HOST pointers, synchronous)
     "deft_lapjv": (C.c_int, [c_fp, C.c_int, C.c_int, C.c_double, c_fp, c_fp, c_fp]),
@@ -196,6 +213,13 @@ class HipLib:
                     ceil = 2500.0 / (6 if self.pieces == 3 else 3)
                     info += " split" + (" patch" if d.p3_kernel in (2, 3) else " halo" if d.p3_kernel else (" x3" if d.x3 else ""))
             prof.append((name, fl, e0, e1, info, nbytes, ceil))
+
+    def value(self, name, *args):
+        """A size-answering entry point: its non-negative value, or the refusal as an error."""
+        n = self._fn[name](*args)
+        if n < 0:
+            raise DeftHipError("%s failed (%d): %s" % (name + self.suffix, n, self.last_error()))
+        return n
 
     def split_arithmetic(self, name, d):
         """Does this launch run on the bf16 matrix instructions (prec 1 honoured)?  The pre-split kernels always do; igemm.hip

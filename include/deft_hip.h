@@ -388,6 +388,66 @@ int deft_conv_direct(const DeftGemmDesc* d, void* stream);
 int deft_split_weights_direct(const float* w, void* w3, int Cout, int Kpad, int KH, int KW, int Cin, void* stream);
 long long deft_direct_weight_bytes(int KH, int KW, int Cin, int Cout);
 
+/* ---- attention-layer operators over tokens (detections or map cells at positions (frame, y, x)) ---------------------------------------
+ * A second kind of sequence model next to deft_lstm_step / deft_motion_step: the tokens of a track's history (or of a clip) as queries, keys
+ * and values.  Rows are [token][head][D] with a token stride `ld*` and a head stride `hs*` in ELEMENTS (views of one projection buffer need no
+ * copy); element type `dtype`: DEFT_F32 / DEFT_F16 / DEFT_BF16, the same for all tensors of a call; every pointer to such rows is 16-byte
+ * aligned and every stride a multiple of 16 bytes.  Forward only, like every entry point of this library. */
+#define DEFT_F32 0
+#define DEFT_F16 1
+#define DEFT_BF16 2
+
+/* Rotary positions with several axes, with or without the RMS norm of every head in the same pass.
+ *   norm != 0:  x <- x * w / sqrt(mean_d x^2 + eps)   per head, in fp32 (w = q_weight / k_weight [D] fp32, NULL = 1)
+ *   pair i < R of a head turns by  angle(t, i) = pos[t][axis[i]] * freq[i]  (formed in double and reduced to a quarter turn before it is
+ *   rounded, so positions far from zero keep their angle):  (x, y) <- (x cos - y sin, y cos + x sin);  inverse != 0: by -angle.
+ *   Pair i is elements (i, i + R), or (2i, 2i + 1) when `adjacent`; elements 2R .. D-1 are not turned.
+ * pos [T][A]: int, or float when pos_float (sub-pixel centres).  q [T][Hq][D] -> q_out, k [T][Hk][D] -> k_out, v [T][Hk][D] -> v_out (copied
+ * only); k and v may be NULL, v needs k.  row != NULL: token t's k / v go to row row[t] of k_out / v_out (a cache with `rows` rows); a row
+ * outside 0 .. rows-1 is not written; two tokens of one call must not name the same row.  q_out = q and (without row) k_out = k are allowed.
+ * One rounding to the element type at the end.  D % 16 == 0 and R % 8 == 0 (fp32: 8 and 4), D <= 256. */
+typedef struct DeftRotary {
+    const void *q, *k, *v;
+    void *q_out, *k_out, *v_out;
+    const void* pos;
+    const double* freq;                /* [R] */
+    const int* axis;                   /* [R], values 0 .. A-1 */
+    const float *q_weight, *k_weight;
+    const int* row;
+    long long ldq, hsq, ldk, hsk, ldv, hsv, ldqo, hsqo, ldko, hsko, ldvo, hsvo;
+    long long rows;
+    int T, Hq, Hk, D, R, A;
+    int dtype, pos_float, adjacent, inverse, norm;
+    float eps;
+} DeftRotary;
+int deft_rotary(const DeftRotary* d, void* stream);
+
+/* Attention over packed sequences of different lengths with grouped heads: query head h reads key / value head h / (Hq / Hk).
+ * Sequence b owns the query rows q_start[b] .. q_start[b+1]-1 (n of them) of q [Tq][Hq][D] and m keys:
+ *   packed (cap == 0): rows k_start[b] .. k_start[b] + m - 1 of k / v [slots][Hk][D]   (k_start NULL: q_start; k_len NULL: m = n)
+ *   cache  (cap > 0):  rows 0 .. m-1 of slot k_start[b] of k / v [slots][cap][Hk][D] (slot strides ssk / ssv), m = k_len[b] -- the single-token
+ *                      form: n = 1 query per track over its history
+ * and query i sees key j when  !causal || j <= m - n + i.  o = softmax(scale * q k^T) v in fp32, rounded once; lse (NULL, or [Tq][Hq]
+ * float) = log of the softmax's sum.  A row that sees no key gets o = 0 and lse = -inf.  Query rows of no sequence are left as they were.  Lengths
+ * and starts are DEVICE data: they are clamped to the tensors (q_start to 0 .. Tq, keys to the rows of the slot / of k), never read past them,
+ * and key rows >= m are never used, whatever they hold; a masked key takes no part even where its value is an infinity or NaN.
+ * max_k is a host-side estimate of the longest m that steers only how the work is split; ws / ws_floats: workspace, at least
+ * deft_attn_ws_floats(d) floats (may be 0: NULL); launches that may overlap need one each.  D = 32, 64, 96 or 128. */
+typedef struct DeftAttn {
+    const void *q, *k, *v;
+    void* o;
+    float* lse;
+    const int *q_start, *k_start, *k_len;
+    float* ws;
+    long long ws_floats;
+    long long ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso, ssk, ssv;
+    int Tq, B, slots, cap, Hq, Hk, D;
+    int dtype, causal, max_k;
+    float scale;
+} DeftAttn;
+int deft_attn(const DeftAttn* d, void* stream);
+long long deft_attn_ws_floats(const DeftAttn* d);
+
 /* ---- host-side association helpers (csrc/assoc.hip): the only entry points that take HOST pointers; synchronous, no stream ---- */
 
 /* matching.linear_assignment's solver (matching.py:40-55: `lap.lapjv(cost_matrix, extend_cost=True, cost_limit=thresh)`; `lap` is a

@@ -13,7 +13,7 @@ OBJCOPY=/opt/rocm/lib/llvm/bin/llvm-objcopy
 [ -x "$OBJCOPY" ] || OBJCOPY=objcopy
 FLAGS="-x c++ -std=c++17 -O2 -g0 -fPIC -pthread -Wno-unused-value -I tests/hipemu"
 pids=""
-for f in igemm igemm3 dcn direct ops pairmlp assoc; do
+for f in igemm igemm3 dcn direct ops pairmlp rotary attn assoc; do
     if [ ! -f $B/o2/$f.o ] || [ deft_amd/csrc/$f.hip -nt $B/o2/$f.o ] || [ deft_amd/csrc/common.h -nt $B/o2/$f.o ] || [ include/deft_hip.h -nt $B/o2/$f.o ] || [ tests/hipemu/hip/hip_runtime.h -nt $B/o2/$f.o ]; then
         X=""; [ $f = assoc ] && X="-ffp-contract=off"
         $CXX $FLAGS $X -c deft_amd/csrc/$f.hip -o $B/o2/$f.o & pids="$pids $!"
@@ -22,8 +22,8 @@ for f in igemm igemm3 dcn direct ops pairmlp assoc; do
 done
 for p in $pids; do wait $p; done
 : > $B/redefine.map
-for f in igemm igemm3 dcn direct ops pairmlp; do nm --defined-only --extern-only $B/o3/$f.o | awk 'NF>=3 {print $NF}'; done | sort -u | awk '{print $1, $1 "_p3"}' > $B/redefine.map
+for f in igemm igemm3 dcn direct ops pairmlp rotary attn; do nm --defined-only --extern-only $B/o3/$f.o | awk 'NF>=3 {print $NF}'; done | sort -u | awk '{print $1, $1 "_p3"}' > $B/redefine.map
 TW=""
-for f in igemm igemm3 dcn direct ops pairmlp; do $OBJCOPY --redefine-syms=$B/redefine.map $B/o3/$f.o $B/o3/$f.twin.o; TW="$TW $B/o3/$f.twin.o"; done
-$CXX -shared -pthread -o $B/libdeft_emu.so $B/o2/igemm.o $B/o2/igemm3.o $B/o2/dcn.o $B/o2/direct.o $B/o2/ops.o $B/o2/pairmlp.o $B/o2/assoc.o $TW
+for f in igemm igemm3 dcn direct ops pairmlp rotary attn; do $OBJCOPY --redefine-syms=$B/redefine.map $B/o3/$f.o $B/o3/$f.twin.o; TW="$TW $B/o3/$f.twin.o"; done
+$CXX -shared -pthread -o $B/libdeft_emu.so $B/o2/igemm.o $B/o2/igemm3.o $B/o2/dcn.o $B/o2/direct.o $B/o2/ops.o $B/o2/pairmlp.o $B/o2/rotary.o $B/o2/attn.o $B/o2/assoc.o $TW
 echo built tests/hipemu/_build/libdeft_emu.so
