@@ -1,108 +1,594 @@
 // Attention over packed sequences of different lengths with grouped heads (DeftAttn, include/deft_hip.h).
 //
-//   s_j = scale * q . k_j over the keys the row sees,  o = sum_j e^(s_j - M) v_j / sum_j e^(s_j - M),  M = max_j s_j
+//   s_j = scale * q . k_j over the keys a row sees,   o = sum_j e^(s_j - M) v_j / sum_j e^(s_j - M)
 //
-// in one pass over the keys: M and the two sums are carried along and multiplied by e^(M_old - M_new) when a larger score comes.  Everything
-// is fp32; the result is rounded once.
+// One pass over the keys: the reference M and both sums are carried along and rescaled when a larger score comes.  A "row" is one (query, head) pair;
+// the G = Hq / Hk heads of a group are rows of the same tile (row r = query r / G, head r % G of the group), so keys and values are read once for
+// the group and a single token still fills G rows.
 //
-// This form: one wave a (query, head) row.  64 keys at a time, a lane forms the score of one key, then the lanes own the columns of o.
+// A wave works on 32 rows with S^T = K Q^T and O^T = V^T P^T (32 x 32 matrix instructions): a lane then owns ONE row (column l & 31) of both, maxima
+// and sums stay inside the lane, and the accumulator of S^T is already laid out as the operand of P^T -- the keys of a 16-key step are merely
+// taken in the order the accumulator holds them, 16 s + 8 (i >> 2) + 4 (l >> 5) + (i & 3), and V's fragments are read in that order too.  P never
+// leaves the registers.  16-bit types: v_mfma_f32_32x32x16, V^T through the transposing LDS read; fp32: v_mfma_f32_32x32x2_f32, exact products.
+//
+// The reference M moves only when a score exceeds it by 2^8 (P <= 2^8 then, harmless in fp32 sums and in 16-bit P): the rescaling of O and the
+// exchange between the two half-waves of a row run on few tiles instead of on all.  fp16 keeps P at 2^6 times its value, so that small
+// probabilities stay out of the subnormals.
+//
+// Two kernels:
+//   attn_prompt_kernel: 128 rows (4 waves x 32), key tiles shared by the waves, double-buffered in LDS by DMA.
+//   attn_step_kernel:   32 rows, the waves take different key tiles, each with its own double-buffered LDS, joined at the end: single tokens
+//                       over long histories, where the keys' bytes are the cost.
+// Both can split the keys over workgroups (partial O, M, L in the workspace, attn_merge_kernel joins them in order).
 #include "common.h"
 
 namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef deft_f32x16 f32x16;
+
+#ifndef DEFT_LDS_TR_HOOK       /* the unit-test SIMT emulator pre-defines these hooks */
+// LDS-DMA of 16 bytes a lane (common.h deft_buffer_load_lds_x4), written out: after the builtin the compiler waits for ALL of a wave's DMA (vmcnt 0)
+// before every transposing LDS read, the next tile's included, and the two-stage loops would not overlap anything.  Nothing is returned to a
+// register; the kernels wait for their pieces themselves.  (One wait state between the write of m0 and its use.)
+typedef u32x4 lds_src;
+typedef unsigned lds_at;
+__device__ __forceinline__ lds_at lds_address(char* lds) { return (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds; }
+// `bytes` from `base` on may be read, chunks behind them arrive as zeros
+__device__ __forceinline__ lds_src lds_source(const char* base, unsigned bytes) {
+    const unsigned long long a = (unsigned long long)base;
+    return lds_src{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)),
+                   (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+__device__ __forceinline__ void lds_fetch(const lds_src& s, lds_at lds, unsigned off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(s) : "memory", "m0");
+}
+// transposing LDS read: the 16 lanes of a group address the rows (i >> 2) x 4-element chunks (i & 3) of a 4 x 16 block; lane i gets column i
+__device__ __forceinline__ s16x4 deft_lds_read_tr16(const void* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(size_t)(__attribute__((address_space(3))) const void*)p);
+}
+__device__ __forceinline__ float deft_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float deft_log2(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ unsigned long long deft_ballot(bool b) { return __ballot(b); }
+#endif
 
 template <int DT> struct Elem;
 template <> struct Elem<DEFT_F32> { typedef float T; };
 template <> struct Elem<DEFT_F16> { typedef _Float16 T; };
 template <> struct Elem<DEFT_BF16> { typedef __bf16 T; };
 
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float M_NONE = -3.0e38f;            // M of a row that has seen no key (finite: -inf - M must not become NaN)
+constexpr float M_SLACK = 8.f;
+
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
-// the sequence of query row t: the last b with q_start[b] <= t; -1 when t belongs to none
-__device__ __forceinline__ int seq_of(const DeftAttn& p, int t) {
-    int lo = 0, hi = p.B;                       // (q_start has B + 1 entries)
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.q_start[mid] <= t) lo = mid; else hi = mid - 1;
+// What a workgroup works on: sequence b, its query rows and keys, and the tile's rows.
+struct Work {
+    int b, hk, split;
+    int q0, n, m;                 // first query, queries, keys
+    int row0, rows;               // first row of the tile, rows of the sequence (n * G)
+    const char *k, *v;            // key 0 / value 0 of this kv head
+};
+
+// Flat tile t -> (sequence, tile of it).  Sequence b starts at flat tile  first(b) = q_start[b] * G / BM + b,  which leaves it at least ceil(n G / BM)
+// tiles whatever the lengths are: no table of lengths is needed on the host, surplus tiles end at once.  64 candidates a step.
+template <int BM>
+__device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, unsigned id, int nsplit, int ntiles, Work& w) {
+    const int G = p.Hq / p.Hk, lane = threadIdx.x & 63;
+    w.hk = (int)(id % (unsigned)p.Hk);                           // neighbouring workgroups (different XCDs) read different heads
+    id /= (unsigned)p.Hk;
+    w.split = nsplit == 1 ? 0 : (int)(id % (unsigned)nsplit);
+    const int t = ntiles - 1 - (int)(nsplit == 1 ? id : id / (unsigned)nsplit);      // causal: the long rows of a sequence first
+    int lo = 0, n = p.B;
+    while (true) {
+        const int step = (n + 63) >> 6, at = lo + lane * step;
+        bool le = false;
+        if (at < lo + n) le = clampi(p.q_start[at], 0, p.Tq) * G / BM + at <= t;      // (Tq * Hq < 2^30)
+        const int c = __popcll(deft_ballot(le));
+        if (c == 0) return false;
+        const int left = n - (c - 1) * step;
+        lo += (c - 1) * step;
+        n = left < step ? left : step;
+        if (n <= 1) break;
     }
-    return lo < p.B && p.q_start[lo] <= t ? lo : -1;
+    const int b = w.b = __builtin_amdgcn_readfirstlane(lo);
+    w.q0 = clampi(p.q_start[b], 0, p.Tq);
+    w.n = clampi(p.q_start[b + 1], 0, p.Tq) - w.q0;
+    if (w.n <= 0) return false;
+    w.rows = w.n * G;
+    const int tile = t - (w.q0 * G / BM + b);
+    if (tile >= (w.rows + BM - 1) / BM) return false;
+    w.row0 = tile * BM;
+    int m = p.k_len ? p.k_len[b] : w.n;
+    const int at = p.k_start ? p.k_start[b] : w.q0;
+    const bool there = at >= 0 && at < p.slots;
+    m = there ? clampi(m, 0, p.cap > 0 ? p.cap : p.slots - at) : 0;
+    w.m = m;
+    const long long ko = m == 0 ? 0 : (long long)at * (p.cap > 0 ? p.ssk : p.ldk), vo = m == 0 ? 0 : (long long)at * (p.cap > 0 ? p.ssv : p.ldv);
+    w.k = (const char*)p.k + (ko + (long long)w.hk * p.hsk) * tsize;
+    w.v = (const char*)p.v + (vo + (long long)w.hk * p.hsv) * tsize;
+    return true;
+}
+// keys the row sees (j < vis)
+__device__ __forceinline__ int visible(const DeftAttn& p, const Work& w, int row, int G) {
+    return p.causal ? clampi(w.m - w.n + row / G + 1, 0, w.m) : w.m;
 }
 
-// rows of the keys of sequence b: their count m, and the element offsets of the first row
-__device__ __forceinline__ int keys_of(const DeftAttn& p, int b, int nq, long long& koff, long long& voff) {
-    int m = p.k_len ? p.k_len[b] : nq;
-    int at = p.k_start ? p.k_start[b] : p.q_start[b];
-    if (p.cap > 0) {
-        m = (at < 0 || at >= p.slots) ? 0 : clampi(m, 0, p.cap);
-        koff = (long long)at * p.ssk;
-        voff = (long long)at * p.ssv;
-    } else {
-        m = (at < 0 || at >= p.slots) ? 0 : clampi(m, 0, p.slots - at);
-        koff = (long long)at * p.ldk;
-        voff = (long long)at * p.ldv;
-    }
-    if (m == 0) koff = voff = 0;
-    return m;
-}
-
-template <int DT>
-__global__ __launch_bounds__(256) void attn_row_kernel(DeftAttn p) {
+// A tile of BN keys in LDS: rows of RB bytes, 16-byte chunks; chunk c of row r sits at slot c ^ f(r).
+//   K is read 16 bytes a lane, 32 rows at one chunk (served in groups of 16 lanes): f spreads the 16 rows of such a group over the 16 slots of the
+//   64 banks.  V of 16-bit types is read by the transposing read, 8 rows x 64 bytes: f_V moves the rows of a half-wave to different 64-byte
+//   groups and the other half-wave's to the other 32 bytes.  V of fp32 is read a row at a time: no conflict to avoid.
+template <int DT, int D>
+struct Tile {
     typedef typename Elem<DT>::T T;
-    constexpr int V = 16 / (int)sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(V)));
-    __shared__ float qs[4][128];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long unit = (long long)blockIdx.x * 4 + wave;
-    const int t = (int)(unit / p.Hq), h = (int)(unit - (long long)t * p.Hq);
-    const int b = t < p.Tq ? seq_of(p, t) : -1;
-    const bool live = b >= 0;
-    if (live)
-        for (int d = lane; d < p.D; d += 64) qs[wave][d] = (float)((const T*)p.q)[(long long)t * p.ldq + (long long)h * p.hsq + d];
-    __syncthreads();
-    if (!live) return;
-    const int q0 = clampi(p.q_start[b], 0, p.Tq), q1 = clampi(p.q_start[b + 1], 0, p.Tq);
-    if (t >= q1) return;
-    long long koff, voff;
-    const int m = keys_of(p, b, q1 - q0, koff, voff);
-    const int hk = h / (p.Hq / p.Hk);
-    const int vis = p.causal ? clampi(m - (q1 - q0) + (t - q0) + 1, 0, m) : m;
-    const T* kp = (const T*)p.k + koff + (long long)hk * p.hsk;
-    const T* vp = (const T*)p.v + voff + (long long)hk * p.hsv;
-    float M = -INFINITY, L = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int j0 = 0; j0 < vis; j0 += 64) {
-        const int j = j0 + lane;
-        float s = -INFINITY;
-        if (j < vis) {
-            const T* kr = kp + (long long)j * p.ldk;
-            float a = 0.f;
-            for (int d = 0; d < p.D; d += V) {
-                const vec x = *(const vec*)(kr + d);
-                for (int e = 0; e < V; ++e) a = fmaf((float)x[e], qs[wave][d + e], a);
+    static constexpr int TS = (int)sizeof(T), RB = D * TS, CPR = RB / 16, NF = CPR / 2, NJ = D / 32;
+    static constexpr float SHIFT = DT == DEFT_F16 ? 6.f : 0.f;
+    typedef T frag_t __attribute__((ext_vector_type(16 / TS)));
+
+    static __device__ __forceinline__ int fk(int r) { return RB % 256 == 0 ? r & 15 : RB % 256 == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+    static __device__ __forceinline__ int fv(int r) {
+        if (DT == DEFT_F32) return 0;
+        const int two = ((r >> 2) & 1) << 1;
+        return RB % 256 == 0 ? ((r & 3) << 2) | two : RB % 256 == 128 ? (((r >> 1) & 1) << 2) | two : two;
+    }
+
+    // Byte offsets (tile-relative) of the chunks this lane fetches; instruction j of the tile deposits 64 consecutive slots.
+    // BN rows in BN * CPR / 64 instructions, instruction first + i * by for i < NI.
+    template <int NI>
+    struct Fetch {
+        unsigned off[NI];
+        template <typename F>
+        __device__ __forceinline__ void init(int lane, int first, int by, long long ld, F f) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int s = (first + i * by) * 64 + lane, r = s / CPR, c = (s - r * CPR) ^ f(r);
+                off[i] = (unsigned)(r * (int)ld) * (unsigned)TS + (unsigned)c * 16u;      // (ld <= 2^22, r < 64: below 2^31)
             }
-            s = a * p.scale;
         }
-        float mx = s;
-        for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-        const float Mn = fmaxf(M, mx), ref = Mn == -INFINITY ? 0.f : Mn;
-        const float al = expf(M - ref), pj = expf(s - ref);
-        float sum = pj;
-        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
-        L = L * al + sum;
-        o0 *= al;
-        o1 *= al;
-        M = Mn;
-        const int nj = vis - j0 < 64 ? vis - j0 : 64;
-        for (int i = 0; i < nj; ++i) {
-            const float w = __shfl(pj, i);
-            const T* vr = vp + (long long)(j0 + i) * p.ldv;
-            if (lane < p.D) o0 = fmaf(w, (float)vr[lane], o0);
-            if (lane + 64 < p.D) o1 = fmaf(w, (float)vr[lane + 64], o1);
+        // rows >= nv arrive as zeros: the range of the source ends with row nv - 1
+        __device__ __forceinline__ void issue(const char* base, lds_at lds, int first, int by, int nv, int row_bytes) const {
+            const lds_src r = lds_source(base, nv <= 0 ? 0u : nv >= 64 ? 0x7FFFFFFFu : (unsigned)((nv - 1) * row_bytes + RB));
+#pragma unroll
+            for (int i = 0; i < NI; ++i) lds_fetch(r, lds + (first + i * by) * 1024, off[i]);
+        }
+    };
+
+    static __device__ __forceinline__ f32x16 zero16() {
+        f32x16 z;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] = 0.f;
+        return z;
+    }
+    static __device__ __forceinline__ f32x16 mfma(frag_t a, frag_t b, f32x16 c) {
+        if constexpr (DT == DEFT_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+            return c;
+        } else if constexpr (DT == DEFT_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+
+    // State of a wave's 32 rows: lane l holds row l & 31 (both half-waves: half of the keys, half of O's columns)
+    struct Rows {
+        frag_t q[NF];                 // chunk 2 j + (l >> 5) of the row
+        f32x16 o[NJ];                 // o[j][r]: column 32 j + 8 (r >> 2) + 4 (l >> 5) + (r & 3)
+        float M, L;                   // scores are kept times scale * log2 e; P = 2^(s - M); L: this half-wave's part
+        __device__ __forceinline__ void init(const T* qrow, int h) {
+#pragma unroll
+            for (int j = 0; j < NF; ++j) q[j] = *(const frag_t*)((const char*)qrow + (2 * j + h) * 16);
+            clear();
+            // (the loads end here: a wait for them inside the loop would wait for the tiles fetched ahead)
+#pragma unroll
+            for (int j = 0; j < NF; ++j) DEFT_OPAQUE(q[j]);
+        }
+        __device__ __forceinline__ void clear() {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[j] = zero16();
+            M = M_NONE;
+            L = 0.f;
+        }
+    };
+
+    // Any infinity or NaN among the BN rows of V?
+    template <int BN>
+    static __device__ __forceinline__ bool any_bad(const char* vs, int lane) {
+        constexpr unsigned EXP = DT == DEFT_F32 ? 0x7f800000u : DT == DEFT_F16 ? 0x7c007c00u : 0x7f807f80u;
+        constexpr unsigned ONE = DT == DEFT_F32 ? 0x00800000u : DT == DEFT_F16 ? 0x04000400u : 0x00800080u;
+        unsigned bad = 0;
+#pragma unroll
+        for (int i = 0; i < BN * CPR / 64; ++i) {
+            if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);       // (16 registers at a time)
+            const u32x4 x = *(const u32x4*)(vs + (i * 64 + lane) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad |= (x[e] & EXP) + ONE;
+        }
+        return deft_ballot((bad & (DT == DEFT_F32 ? 0x80000000u : 0x80008000u)) != 0) != 0;
+    }
+    // One tile of BN = 32 NT keys for a wave: ks, vs the tile in LDS; vis: keys of the tile this lane's row sees (may be <= 0 or > BN); `partial`
+    // (wave-uniform): some row does not see all of them; `hidden`: some row does not see keys that are there (their values must not reach it).
+    // Returns whether such hidden values are infinite or NaN: the wave's result is not valid then, and its pass is run again with CAREFUL.
+    template <int NT, bool CAREFUL>
+    static __device__ __forceinline__ bool step(Rows& w, const char* ks, const char* vs, int vis, bool partial, bool hidden, float sc, int lane) {
+        const int h = lane >> 5;
+        f32x16 s[NT];
+        {
+            const int key = lane & 31;                                         // rows 32 t + key: f(32 t + key) = f(key)
+            const int x = h ^ fk(key);
+            const char* const kr = ks + key * RB;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[t] = zero16();
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) s[t] = mfma(*(const frag_t*)(kr + t * 32 * RB + (((2 * j) ^ x) << 4)), w.q[j], s[t]);
+        }
+        if (partial) {
+            const int lim = vis - 4 * h;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) < lim ? s[t][r] : -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+        if (deft_ballot(mx * sc > w.M + (SHIFT + M_SLACK)) != 0) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float Mn = fmaxf(w.M, mx * sc - SHIFT);
+            const float al = deft_exp2(w.M - Mn);
+            w.M = Mn;
+            w.L *= al;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) w.o[j][r] *= al;
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = deft_exp2(fmaf(s[t][r], sc, -w.M));
+                s[t][r] = e;
+                sum[r & 3] += e;
+            }
+        w.L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if constexpr (CAREFUL) {
+            careful<NT>(w, s, vs, vis, lane);
+            return false;
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const pfrag_t pb = probs(s[t], g);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) w.o[j] = pv(value(vs, t, g, j, lane), pb, w.o[j]);
+                }
+            return hidden && any_bad<32 * NT>(vs, lane);
+        }
+    }
+
+    // ---- the products with V, 16 / TS keys a half-wave at a time: group g of a 32-key block holds the accumulator registers GK g .. GK g + GK - 1
+    static constexpr int GK = DT == DEFT_F32 ? 4 : 8, NG = 16 / GK;
+    typedef T pfrag_t __attribute__((ext_vector_type(GK)));
+    static __device__ __forceinline__ pfrag_t probs(const f32x16& s, int g) {
+        pfrag_t p;
+#pragma unroll
+        for (int e = 0; e < GK; ++e) p[e] = (T)s[GK * g + e];
+        return p;
+    }
+    // this lane's fragment of V^T: column 32 j + (l & 31), the keys of probs() of group g of block t
+    static __device__ __forceinline__ pfrag_t value(const char* vs, int t, int g, int j, int lane) {
+        const int h = lane >> 5;
+        if constexpr (DT == DEFT_F32) {
+            pfrag_t v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = *(const float*)(vs + (32 * t + 8 * g + 4 * h + e) * RB + (32 * j + (lane & 31)) * 4);
+            return v;
+        } else {
+            const int i = lane & 15, row = 4 * h + (i >> 2), c0 = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+            const char* const a = vs + row * RB + (i & 1) * 8 + (32 * t + 16 * g) * RB + (((4 * j + c0) ^ fv(row)) << 4);      // f(row + 8 x) = f(row)
+            return __builtin_bit_cast(pfrag_t, __builtin_shufflevector(deft_lds_read_tr16(a), deft_lds_read_tr16(a + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+    static __device__ __forceinline__ f32x16 pv(pfrag_t v, pfrag_t p, f32x16 o) {
+        if constexpr (DT == DEFT_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e], p[e], o, 0, 0, 0);
+            return o;
+        } else return mfma(v, p, o);
+    }
+    // Products for tiles with infinities or NaN among values that not every row may see (0 * inf is NaN in a product): the finite values with P,
+    // then, with P replaced by what is visible, how many +inf / NaN and how many -inf / NaN each row sees -- what is seen is added.
+    template <int NT>
+    static __device__ __forceinline__ void careful(Rows& w, f32x16 (&s)[NT], const char* vs, int vis, int lane) {
+        const int lim = vis - 4 * (lane >> 5);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const pfrag_t p = probs(s[t], g);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    pfrag_t v = value(vs, t, g, j, lane);
+#pragma unroll
+                    for (int e = 0; e < GK; ++e) v[e] = (float)v[e] - (float)v[e] == 0.f ? v[e] : (T)0.f;
+                    w.o[j] = pv(v, p, w.o[j]);
+                }
+            }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[t][r] = 32 * t + 8 * (r >> 2) + (r & 3) < lim ? 1.f : 0.f;
+#pragma unroll 1
+        for (float sign = 1.f; sign >= -1.f; sign -= 2.f) {
+            int l = lane;
+            DEFT_OPAQUE_NV(l);                                       // (no fragment is kept over the two passes: registers)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                f32x16 acc = zero16();
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        __builtin_amdgcn_sched_barrier(0);           // (nor fetched ahead)
+                        pfrag_t v = value(vs, t, g, j, l);
+#pragma unroll
+                        for (int e = 0; e < GK; ++e) v[e] = (float)v[e] * sign <= 3.4028235e38f ? (T)0.f : (T)1.f;
+                        acc = pv(v, probs(s[t], g), acc);
+                    }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) w.o[j][r] = acc[r] > 0.f ? w.o[j][r] + sign * INFINITY : w.o[j][r];
+            }
+        }
+    }
+};
+
+// Where a split's partial results stand in the workspace: O [split][row][D], then (M, L) [split][row]; row = query * Hq + head
+__device__ __forceinline__ size_t ws_row(const DeftAttn& p, int split, int query, int head) { return ((size_t)split * p.Tq + query) * p.Hq + head; }
+__device__ __forceinline__ float* ws_ml(const DeftAttn& p, int nsplit) { return p.ws + (size_t)nsplit * p.Tq * p.Hq * p.D; }
+
+constexpr int BM = 128;
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, int nsplit, int ntiles) {
+    typedef Tile<DT, D> TL;
+    typedef typename TL::T T;
+    constexpr int NT = DT == DEFT_F32 ? 1 : 2, BN = 32 * NT, KB = BN * TL::RB, NI = BN * TL::CPR / 256;
+    static_assert(NI * 256 == BN * TL::CPR, "whole DMA instructions");
+    __shared__ __attribute__((aligned(1024))) char lds[4 * KB];                    // K, K, V, V
+    __shared__ int again;
+    const int G = p.Hq / p.Hk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    Work w;
+    if (!find_work<BM>(p, TL::TS, blockIdx.x, nsplit, ntiles, w)) return;
+    const float sc = p.scale * LOG2E;
+    const int wr0 = w.row0 + wave * 32, row = wr0 + (lane & 31);
+    const int rc = row < w.rows ? row : w.rows - 1, query = w.q0 + rc / G, head = w.hk * G + rc % G;
+    const bool on = wr0 < w.rows;                                                  // this wave has rows
+    const int last = w.rows - 1;
+    const int vis = visible(p, w, rc, G);
+    const int vmin = __builtin_amdgcn_readfirstlane(visible(p, w, wr0 < last ? wr0 : last, G));               // the wave's first and last row
+    const int vmax = __builtin_amdgcn_readfirstlane(visible(p, w, wr0 + 31 < last ? wr0 + 31 : last, G));
+    const int bmax = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0 + BM - 1 < last ? w.row0 + BM - 1 : last, G));
+    const int nt = (bmax + BN - 1) / BN, per = (nt + nsplit - 1) / nsplit;
+    const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
+
+    typename TL::Rows rw;
+    rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
+    typename TL::template Fetch<NI> fk, fv;
+    fk.init(lane, wave, 4, p.ldk, [](int r) { return TL::fk(r); });
+    fv.init(lane, wave, 4, p.ldv, [](int r) { return TL::fv(r); });
+    const int kr = (int)p.ldk * TL::TS, vr = (int)p.ldv * TL::TS;                  // bytes between keys (<= 2^24)
+    const lds_at base = lds_address(lds);
+    auto issue = [&](int t) {
+        const int nv = w.m - t * BN;
+        fk.issue(w.k + (long long)t * BN * kr, base + (t & 1) * KB, wave, 4, nv, kr);
+        fv.issue(w.v + (long long)t * BN * vr, base + 2 * KB + (t & 1) * KB, wave, 4, nv, vr);
+    };
+    if (tid == 0) again = 0;
+    if (t0 < t1) issue(t0);
+    for (int t = t0; t < t1; ++t) {
+        DEFT_PIPE_BARRIER(0);                                                      // tile t is here, and nobody reads tile t - 1 any more
+        if (t + 1 < t1) issue(t + 1);
+        const int k0 = t * BN;
+        if (on && k0 < vmax) {
+            const int end = k0 + BN < w.m ? k0 + BN : w.m;
+            if (TL::template step<NT, false>(rw, lds + (t & 1) * KB, lds + 2 * KB + (t & 1) * KB, vis - k0, vmin < k0 + BN, vmin < end, sc, lane)) again = 1;
+        }
+    }
+    if (p.causal) {
+        __syncthreads();
+        if (again) {                                                               // (rare: infinities or NaN behind the diagonal of some row)
+            rw.clear();
+            for (int t = t0; t < t1; ++t) {
+                __syncthreads();
+                issue(t);
+                DEFT_PIPE_BARRIER(0);
+                if (on && t * BN < vmax) TL::template step<NT, true>(rw, lds + (t & 1) * KB, lds + 2 * KB + (t & 1) * KB, vis - t * BN, true, false, sc, lane);
+            }
+        }
+    }
+    rw.L += __shfl_xor(rw.L, 32);
+    if (nsplit > 1) {
+        if (row < w.rows) {
+            float* const op = p.ws + ws_row(p, w.split, query, head) * D;
+#pragma unroll
+            for (int j = 0; j < TL::NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) *(f32x4*)(op + 32 * j + 2 * r + 4 * h) = f32x4{rw.o[j][r], rw.o[j][r + 1], rw.o[j][r + 2], rw.o[j][r + 3]};
+            if (h == 0) {
+                float* const ml = ws_ml(p, nsplit) + ws_row(p, w.split, query, head) * 2;
+                ml[0] = rw.M;
+                ml[1] = rw.L;
+            }
+        }
+        return;
+    }
+    const float inv = rw.L == 0.f ? 0.f : 1.f / rw.L;
+    if (row < w.rows) {
+        T* const op = (T*)p.o + (long long)query * p.ldo + (long long)head * p.hso;
+        typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int j = 0; j < TL::NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                t4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (T)(rw.o[j][r + e] * inv);
+                *(t4*)(op + 32 * j + 2 * r + 4 * h) = x;
+            }
+        if (p.lse && h == 0) p.lse[(long long)query * p.Hq + head] = rw.L == 0.f ? -INFINITY : (rw.M + deft_log2(rw.L)) * LN2;
+    }
+}
+
+template <int DT, int D>
+struct StepCfg {
+    typedef Tile<DT, D> TL;
+    static constexpr int NW = TL::RB > 256 ? 2 : 4;               // waves: two 32-key stages of K and V each stay within 128 KB
+    static constexpr int KB = 32 * TL::RB, LDS = NW * 4 * KB;
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__(64 * (StepCfg<DT, D>::NW)) void attn_step_kernel(DeftAttn p, int nsplit, int ntiles) {
+    typedef Tile<DT, D> TL;
+    typedef typename TL::T T;
+    typedef StepCfg<DT, D> C;
+    constexpr int NW = C::NW, KB = C::KB, NI = TL::CPR / 2;
+    static_assert(C::LDS >= NW * 32 * D * 4, "the join fits the stages");
+    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    __shared__ float ms[NW][32], ls[NW][32];
+    const int G = p.Hq / p.Hk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
+    Work w;
+    if (!find_work<32>(p, TL::TS, blockIdx.x, nsplit, ntiles, w)) return;
+    const float sc = p.scale * LOG2E;
+    const int last = w.rows - 1, row = w.row0 + l32, rc = row < last ? row : last;
+    const int query = w.q0 + rc / G, head = w.hk * G + rc % G;
+    const int vis = visible(p, w, rc, G);
+    const int vmin = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0, G));
+    const int vmax = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0 + 31 < last ? w.row0 + 31 : last, G));
+    const int nt = (vmax + 31) >> 5, per = (nt + nsplit - 1) / nsplit;
+    const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
+
+    typename TL::Rows rw;
+    rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
+    typename TL::template Fetch<NI> fk, fv;
+    fk.init(lane, 0, 1, p.ldk, [](int r) { return TL::fk(r); });
+    fv.init(lane, 0, 1, p.ldv, [](int r) { return TL::fv(r); });
+    char* const mine = lds + wave * 4 * KB;                                        // K, V of stage 0, K, V of stage 1
+    const int kr = (int)p.ldk * TL::TS, vr = (int)p.ldv * TL::TS;                  // bytes between keys (<= 2^24)
+    const lds_at base = lds_address(mine);
+    auto issue = [&](int t, int st) {
+        const int nv = w.m - t * 32;
+        fk.issue(w.k + 32ll * t * kr, base + st * 2 * KB, 0, 1, nv, kr);
+        fv.issue(w.v + 32ll * t * vr, base + st * 2 * KB + KB, 0, 1, nv, vr);
+    };
+    int st = 0, again = 0;
+    if (t0 + wave < t1) issue(t0 + wave, 0);
+    if (t0 + wave + NW < t1) issue(t0 + wave + NW, 1);
+    for (int t = t0 + wave; t < t1; t += NW, st ^= 1) {
+        if (t + NW < t1) { DEFT_WAVE_VM(2 * NI); } else { DEFT_WAVE_VM(0); }       // this wave's tile t is here (the stages are its own: no barrier)
+        const int k0 = t * 32, end = k0 + 32 < w.m ? k0 + 32 : w.m;
+        if (TL::template step<1, false>(rw, mine + st * 2 * KB, mine + st * 2 * KB + KB, vis - k0, vmin < k0 + 32, vmin < end, sc, lane)) again = 1;
+        if (t + 2 * NW < t1) {
+            DEFT_WAVE_LGKM();                                                      // its reads have returned: the stage may be filled again
+            issue(t + 2 * NW, st);
+        }
+    }
+    if (again) {                                                                   // (rare: infinities or NaN behind the diagonal of some row)
+        rw.clear();
+        for (int t = t0 + wave; t < t1; t += NW) {
+            DEFT_WAVE_LGKM();
+            issue(t, 0);
+            DEFT_WAVE_VM(0);
+            TL::template step<1, true>(rw, mine, mine + KB, vis - t * 32, true, false, sc, lane);
+        }
+    }
+    // join the waves: everybody's M and L, then O scaled to the common M, summed in wave order
+    rw.L += __shfl_xor(rw.L, 32);
+    if (h == 0) { ms[wave][l32] = rw.M; ls[wave][l32] = rw.L; }
+    __syncthreads();
+    float M = ms[0][l32];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) M = fmaxf(M, ms[i][l32]);
+    const float al = deft_exp2(rw.M - M);
+    float* const os = (float*)lds;                                                 // [wave][column][32 rows]
+#pragma unroll
+    for (int j = 0; j < TL::NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) os[(wave * D + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + l32] = rw.o[j][r] * al;
+    __syncthreads();
+    // thread: a row's chunk of 4 columns
+    const int nrows = w.rows - w.row0 < 32 ? w.rows - w.row0 : 32;
+    for (int it = tid; it < nrows * (D / 4); it += 64 * NW) {
+        const int r = it / (D / 4), c = (it - r * (D / 4)) * 4;
+        float Mr = ms[0][r];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) Mr = fmaxf(Mr, ms[i][r]);
+        float Lr = 0.f;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            Lr += ls[i][r] * deft_exp2(ms[i][r] - Mr);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += os[(i * D + c + e) * 32 + r];
+        }
+        const int qr = w.q0 + (w.row0 + r) / G, hd = w.hk * G + (w.row0 + r) % G;
+        if (nsplit > 1) {
+            *(f32x4*)(p.ws + ws_row(p, w.split, qr, hd) * D + c) = x;
+            if (c == 0) {
+                float* const ml = ws_ml(p, nsplit) + ws_row(p, w.split, qr, hd) * 2;
+                ml[0] = Mr;
+                ml[1] = Lr;
+            }
+        } else {
+            const float inv = Lr == 0.f ? 0.f : 1.f / Lr;
+            typedef T t4 __attribute__((ext_vector_type(4)));
+            t4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
+            *(t4*)((T*)p.o + (long long)qr * p.ldo + (long long)hd * p.hso + c) = y;
+            if (p.lse && c == 0) p.lse[(long long)qr * p.Hq + hd] = Lr == 0.f ? -INFINITY : (Mr + deft_log2(Lr)) * LN2;
+        }
+    }
+}
+
+// Joins the splits of a row, in order: one wave a row.  Rows of no sequence have no partials and are not written.
+template <int DT>
+__global__ __launch_bounds__(256) void attn_merge_kernel(DeftAttn p, int nsplit) {
+    typedef typename Elem<DT>::T T;
+    const int lane = threadIdx.x & 63;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int q = (int)(row / p.Hq), h = (int)(row - (long long)q * p.Hq);
+    if (q >= p.Tq || q < p.q_start[0] || q >= p.q_start[p.B]) return;
+    const float* const ml = ws_ml(p, nsplit);
+    float M = M_NONE;
+    for (int s = 0; s < nsplit; ++s) M = fmaxf(M, ml[ws_row(p, s, q, h) * 2]);
+    float L = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int s = 0; s < nsplit; ++s) {
+        const size_t at = ws_row(p, s, q, h);
+        const float al = deft_exp2(ml[at * 2] - M), l = ml[at * 2 + 1];
+        if (l == 0.f) continue;                                    // saw no key
+        L = fmaf(l, al, L);
+        if (lane * 2 < p.D) {
+            const float2 x = *(const float2*)(p.ws + at * p.D + lane * 2);
+            o0 = fmaf(x.x, al, o0);
+            o1 = fmaf(x.y, al, o1);
         }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    T* op = (T*)p.o + (long long)t * p.ldo + (long long)h * p.hso;
-    if (lane < p.D) op[lane] = (T)(o0 * inv);
-    if (lane + 64 < p.D) op[lane + 64] = (T)(o1 * inv);
-    if (p.lse && lane == 0) p.lse[(long long)t * p.Hq + h] = M + logf(L);
+    if (lane * 2 < p.D) {
+        T* const op = (T*)p.o + (long long)q * p.ldo + (long long)h * p.hso + lane * 2;
+        typedef T t2 __attribute__((ext_vector_type(2)));
+        const t2 y = {(T)(o0 * inv), (T)(o1 * inv)};
+        *(t2*)op = y;
+    }
+    if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + deft_log2(L)) * LN2;
 }
 
 bool in_fits(long long ld, long long hs, int V) { return ld % V == 0 && hs % V == 0 && ld >= 0 && hs >= 0; }
@@ -113,33 +599,80 @@ int attn_check(const DeftAttn* d) {
     DEFT_CHECK(d->D == 32 || d->D == 64 || d->D == 96 || d->D == 128, -132, "deft_attn: D=%d (32, 64, 96 or 128)", d->D);
     DEFT_CHECK(d->Hk > 0 && d->Hq > 0 && d->Hq % d->Hk == 0 && d->Hq <= 4096, -133, "deft_attn: Hq=%d is not a multiple of Hk=%d", d->Hq, d->Hk);
     DEFT_CHECK(d->Tq >= 0 && d->B >= 0 && d->slots >= 0 && d->cap >= 0, -134, "deft_attn: Tq=%d B=%d slots=%d cap=%d", d->Tq, d->B, d->slots, d->cap);
-    DEFT_CHECK((long long)d->Tq * d->Hq < (1ll << 31) && (long long)d->B * d->Hk < (1ll << 31), -134, "deft_attn: Tq * Hq must stay below 2^31");
+    DEFT_CHECK((long long)d->Tq * d->Hq < (1ll << 30) && (long long)d->B * d->Hk < (1ll << 24), -134, "deft_attn: Tq=%d x Hq=%d rows, B=%d (below 2^30, 2^24 / Hk)", d->Tq, d->Hq, d->B);
     DEFT_CHECK(d->cap == 0 || (d->k_start && d->k_len), -135, "deft_attn: a cache (cap=%d) needs k_start (slots) and k_len", d->cap);
     const int V = d->dtype == DEFT_F32 ? 4 : 8;
     DEFT_CHECK((((size_t)d->q | (size_t)d->k | (size_t)d->v | (size_t)d->o) & 15) == 0, -136, "deft_attn: pointers must be 16-byte aligned");
     DEFT_CHECK(in_fits(d->ldq, d->hsq, V) && in_fits(d->ldk, d->hsk, V) && in_fits(d->ldv, d->hsv, V) && in_fits(d->ldo, d->hso, V) &&
                    in_fits(d->ssk, d->ssv, V) && (d->Tq <= 1 || d->ldo >= d->D) && (d->Hq <= 1 || d->hso >= d->D),
-               -137, "deft_attn: strides must be multiples of %d elements, and the rows of o apart", V);
+               -137, "deft_attn: strides must be multiples of %d elements and keep the rows of o apart", V);
     DEFT_CHECK(d->ldk <= (1 << 22) && d->ldv <= (1 << 22), -137, "deft_attn: ldk=%lld ldv=%lld (at most 2^22 elements between tokens)", d->ldk, d->ldv);
+    DEFT_CHECK(d->scale > 0.f && d->scale < INFINITY, -138, "deft_attn: scale=%g must be positive", (double)d->scale);
     return 0;
+}
+
+// How a call runs: the kernel, its flat tiles, and over how many workgroups the keys of a tile are split.
+struct Choice { bool step; int nsplit, ntiles; };
+Choice choose(const DeftAttn* d) {
+    const int G = d->Hq / d->Hk;
+    Choice c;
+    c.step = (long long)d->Tq * G <= 32ll * d->B;                  // up to 32 rows a sequence on average
+    const int bm = c.step ? 32 : BM;
+    c.ntiles = d->Tq * G / bm + d->B;                              // (below 2^26 + 2^24)
+    // rows that are there fill about this many workgroups
+    const long long busy = ((long long)d->Tq * G / bm + (c.step ? d->B : d->B / 2 + 1)) * d->Hk;
+    const int keys = c.step ? 256 : 512;                           // keys a split should have at least
+    long long want = busy < 512 ? (1024 + busy - 1) / busy : 1;
+    const long long most = ((long long)d->max_k + keys - 1) / keys;
+    if (want > most) want = most;
+    if (want > 64) want = 64;
+    c.nsplit = want < 1 ? 1 : (int)want;
+    return c;
+}
+
+template <int DT, int D>
+void attn_launch(const DeftAttn& d, const Choice& c, unsigned grid, hipStream_t s) {
+    if (c.step) hipLaunchKernelGGL((attn_step_kernel<DT, D>), dim3(grid), dim3(64 * StepCfg<DT, D>::NW), 0, s, d, c.nsplit, c.ntiles);
+    else hipLaunchKernelGGL((attn_prompt_kernel<DT, D>), dim3(grid), dim3(256), 0, s, d, c.nsplit, c.ntiles);
+}
+template <int DT>
+void attn_launch_d(const DeftAttn& d, const Choice& c, unsigned grid, hipStream_t s) {
+    switch (d.D) {
+        case 32: attn_launch<DT, 32>(d, c, grid, s); break;
+        case 64: attn_launch<DT, 64>(d, c, grid, s); break;
+        case 96: attn_launch<DT, 96>(d, c, grid, s); break;
+        default: attn_launch<DT, 128>(d, c, grid, s);
+    }
+    if (c.nsplit > 1) {
+        const unsigned mg = (unsigned)(((long long)d.Tq * d.Hq + 3) / 4);
+        hipLaunchKernelGGL((attn_merge_kernel<DT>), dim3(mg), dim3(256), 0, s, d, c.nsplit);
+    }
 }
 
 }  // namespace
 
 extern "C" long long deft_attn_ws_floats(const DeftAttn* d) {
     const int rc = attn_check(d);
-    return rc < 0 ? rc : 0;
+    if (rc < 0) return rc;
+    if (d->Tq == 0 || d->B == 0) return 0;
+    const Choice c = choose(d);
+    return c.nsplit > 1 ? (long long)c.nsplit * d->Tq * d->Hq * (d->D + 2) : 0;
 }
 
 extern "C" int deft_attn(const DeftAttn* d, void* stream) {
     const int rc = attn_check(d);
     if (rc < 0) return rc;
     if (d->Tq == 0 || d->B == 0) return 0;
-    const unsigned grid = (unsigned)(((long long)d->Tq * d->Hq + 3) / 4);
+    const Choice c = choose(d);
+    const long long need = c.nsplit > 1 ? (long long)c.nsplit * d->Tq * d->Hq * (d->D + 2) : 0;
+    DEFT_CHECK(need == 0 || (d->ws && d->ws_floats >= need && ((size_t)d->ws & 15) == 0), -139, "deft_attn: workspace of %lld floats, 16-byte aligned, has %lld", need,
+               d->ws ? d->ws_floats : 0ll);
+    const long long grid = (long long)c.ntiles * c.nsplit * d->Hk;
+    DEFT_CHECK(grid < (1ll << 31), -134, "deft_attn: %lld workgroups", grid);
     hipStream_t s = (hipStream_t)stream;
-    if (d->dtype == DEFT_F32) hipLaunchKernelGGL((attn_row_kernel<DEFT_F32>), dim3(grid), dim3(256), 0, s, *d);
-    else if (d->dtype == DEFT_F16) hipLaunchKernelGGL((attn_row_kernel<DEFT_F16>), dim3(grid), dim3(256), 0, s, *d);
-    else hipLaunchKernelGGL((attn_row_kernel<DEFT_BF16>), dim3(grid), dim3(256), 0, s, *d);
+    if (d->dtype == DEFT_F32) attn_launch_d<DEFT_F32>(*d, c, (unsigned)grid, s);
+    else if (d->dtype == DEFT_F16) attn_launch_d<DEFT_F16>(*d, c, (unsigned)grid, s);
+    else attn_launch_d<DEFT_BF16>(*d, c, (unsigned)grid, s);
     DEFT_CHECK_LAUNCH("attn");
     return 0;
 }

@@ -186,6 +186,9 @@ __device__ __forceinline__ void deft_buffer_load_lds_x4s(deft_rsrc_t r, void* ld
 // rendezvous the workgroup (raw s_barrier: __syncthreads() would drain vmcnt to 0 while a DMA is outstanding).  The
 // empty asm statements keep the compiler from moving LDS accesses across it.
 #define DEFT_WAIT_VM(N) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory")
+// wave-private LDS stages (attn.hip) need no barrier: a wave waits for its own DMA pieces, and for its own LDS reads before it fills a stage again
+#define DEFT_WAVE_VM(N) DEFT_WAIT_VM(N)
+#define DEFT_WAVE_LGKM() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
 // lgkmcnt(0): this wave's LDS reads have RETURNED before it arrives.  The compiler may sink MFMAs (not memory operations) below
 // the barrier together with the wait for their ds_read operands; another wave's DMA into the stage those reads target would
 // then race with them (seen on the hardware as rare wrong tiles in the one-stage loop).

@@ -500,6 +500,41 @@ static inline void deft_buffer_load_lds_x4s(deft_rsrc_t r, void* lds_wave_base, 
 #define DEFT_PIPE_BARRIER(N) do { hipemu::dma_wait(N); hipemu::yield(hipemu::Y_BLOCK); } while (0)
 #define DEFT_PIPE_BARRIER_ONLY() hipemu::yield(hipemu::Y_BLOCK)
 #define DEFT_WAIT_VM(N) hipemu::dma_wait(N)
+// (the lanes of a wave run one after another here: meet before another lane's pieces are read, or overwritten)
+#define DEFT_WAVE_VM(N) do { hipemu::dma_wait(N); hipemu::yield(hipemu::Y_WAVE); } while (0)
+#define DEFT_WAVE_LGKM() hipemu::yield(hipemu::Y_WAVE)
+// hooks of deft_amd/csrc/attn.hip: the transposing 16-bit LDS read (lane i of a group of 16 gets column i of the 4 x 16 block whose row (j >> 2),
+// 4-element chunk (j & 3) lane j addresses), ballot, base-2 exponential and logarithm
+#define DEFT_LDS_TR_HOOK 1
+typedef short hipemu_s16x4 __attribute__((ext_vector_type(4)));
+static inline hipemu_s16x4 deft_lds_read_tr16(const void* ptr) {
+    hipemu::State& s = hipemu::S();
+    const int p = s.parity ^ 1, lane = s.lane;
+    short v[4];
+    memcpy(v, ptr, 8);
+    for (int e = 0; e < 4; ++e) s.xf[p][e][lane] = (float)v[e];
+    hipemu::yield(hipemu::Y_WAVE);
+    hipemu::State& t = hipemu::S();
+    const int g = lane & ~15, i = lane & 15;
+    hipemu_s16x4 r;
+    for (int e = 0; e < 4; ++e) r[e] = (short)t.xf[p][i & 3][g + 4 * e + (i >> 2)];
+    return r;
+}
+typedef deft_rsrc_t lds_src;
+typedef char* lds_at;
+static inline lds_at lds_address(char* lds) { return lds; }
+static inline lds_src lds_source(const char* base, unsigned bytes) { return lds_src{base, bytes}; }
+static inline void lds_fetch(const lds_src& s, lds_at lds, unsigned off) { deft_buffer_load_lds_x4(s, (float*)lds, off); }
+static inline unsigned long long deft_ballot(bool b) {
+    const float *A, *B;
+    hipemu::exchange(b ? 1.f : 0.f, 0.f, A, B);
+    unsigned long long m = 0;
+    for (int l = 0; l < 64; ++l) m |= (unsigned long long)(A[l] != 0.f) << l;
+    return m;
+}
+static inline float deft_exp2(float x) { return exp2f(x); }
+static inline float deft_log2(float x) { return log2f(x); }
+static inline int __popcll(unsigned long long x) { return __builtin_popcountll(x); }
 extern "C" __attribute__((weak, visibility("default"))) void hipemu_set_late_dma(int on) { hipemu::late_dma() = on; }
 #define DEFT_OPAQUE(v) ((void)(v))
 #define DEFT_OPAQUE_NV(v) ((void)(v))

@@ -48,13 +48,25 @@ SHAPES = [
     dict(nq=[1, 1, 1], nk=[66, 1, 0], H=6, Hk=2, D=64, cache="slots", poison=True),
     dict(nq=[9, 1], nk=[130, 5], H=3, Hk=1, D=32, cache="slots", poison=True),
     dict(nq=[6, 3], nk=[6, 3], H=2, Hk=1, D=64, gap=5, poison=True, head_major=True),
+    dict(nq=[150], nk=[190], H=1, Hk=1, D=64),                                 # several tiles of keys and of rows
+    dict(nq=[1, 2], nk=[600, 300], H=2, Hk=1, D=32, cache="slots", poison=True),   # split keys, joined
+    dict(nq=[70], nk=[1100], H=1, Hk=1, D=32),                                 # the same for a prompt
+    dict(nq=[1], nk=[520], H=5, Hk=1, D=128, cache="slots"),
 ]
+
+
+@pytest.fixture(params=["early", "late"])
+def dma(emu_lib, request):
+    """LDS-DMA pieces delivered when they are issued, or only when their wave waits for them."""
+    emu_lib.cdll.hipemu_set_late_dma(int(request.param == "late"))
+    yield emu_lib
+    emu_lib.cdll.hipemu_set_late_dma(0)
 
 
 @pytest.mark.parametrize("dt", [F32, F16, BF16])
 @pytest.mark.parametrize("kw", SHAPES)
-def test_attend(emu_lib, dt, kw):
-    ac.check_attend(emu_lib, "cpu", dt, **kw)
+def test_attend(dma, dt, kw):
+    ac.check_attend(dma, "cpu", dt, **kw)
 
 
 def _poison_last_keys(bad):
