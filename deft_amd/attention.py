@@ -12,16 +12,21 @@ buffer need no copy).  Every call is asynchronous on the current stream of the p
 stream-ordered allocator, so calls on several streams and captured graphs share nothing.  Forward only, like the rest of the package; refusals raise
 DeftHipError.
 """
-import ctypes as C
 import math
+import struct
 
 import torch
 
-from . import hiplib
 from .engine import _Plan
-from .hiplib import AttnDesc, DeftHipError, RotaryDesc
+from .hiplib import DeftHipError, _raw_stream
 
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_current_device = torch.cuda.current_device
+# DeftRotary and DeftAttn packed in one call each (field order and layout of hiplib.RotaryDesc / AttnDesc): a call's host time is what counts where a
+# launch is a few microseconds, and setting forty ctypes fields one by one costs as much as such a launch
+_ROTARY = struct.Struct("@12P13q11if0q")
+_ATTN = struct.Struct("@9P11q10if0q")
+_SPLIT_KEYS = 256          # no kernel splits the keys of a row below this many (csrc/attn.hip choose()): no workspace to ask for
 
 
 def _refuse(cond, *msg):
@@ -44,7 +49,8 @@ class AttentionPlan(_Plan):
         self.heads, self.kv_heads, self.head_dim = int(heads), int(kv_heads), int(head_dim)
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
         self.eps, self.adjacent = float(eps), bool(adjacent)
-        self.device = torch.empty(0, device=self.device).device          # with its index: tensors and launches belong to THIS device
+        at = torch.empty(0, device=self.device)                          # (with its index: tensors and launches belong to THIS device)
+        self.device, self._index = at.device, at.get_device()            # -1: host memory, the unit-test build
         self.pairs = 0
         if axes is not None:
             axes = [int(n) for n in axes]
@@ -57,7 +63,10 @@ class AttentionPlan(_Plan):
             _refuse(tuple(f.shape) != (self.pairs,), "freq: one value for each of the %d pairs", self.pairs)
             self.freq = self.dev(f)
             self.axis = self.dev(torch.tensor(axis, dtype=torch.int32))
+            self._freq_ptr, self._axis_ptr = self.freq.data_ptr(), self.axis.data_ptr()
         self.q_weight, self.k_weight = self._weight("q_weight", q_weight), self._weight("k_weight", k_weight)
+        self._qw_ptr = 0 if self.q_weight is None else self.q_weight.data_ptr()
+        self._kw_ptr = 0 if self.k_weight is None else self.k_weight.data_ptr()
 
     def _weight(self, name, w):
         if w is None:
@@ -65,30 +74,52 @@ class AttentionPlan(_Plan):
         _refuse(tuple(w.shape) != (self.head_dim,), "%s has shape %s, wanted [%d]", name, tuple(w.shape), self.head_dim)
         return self.dev(w.detach().to(torch.float32).clone())
 
-    def _rows(self, name, x, heads, dtype, tokens=None, ndim=3):
-        """Refuses what is not [tokens][heads][head_dim] (ndim 4: [slots][rows][heads][head_dim]) rows of `dtype` on the plan's device."""
-        _refuse(not isinstance(x, torch.Tensor), "%s is not a tensor", name)
-        shape = x.shape
-        _refuse(len(shape) != ndim or shape[-2] != heads or shape[-1] != self.head_dim, "%s has shape %s, wanted %s[%d][%d]", name, tuple(shape),
-                "[tokens]" if ndim == 3 else "[slots][rows]", heads, self.head_dim)
-        _refuse(x.dtype is not dtype, "%s is %s, wanted %s", name, x.dtype, dtype)
-        _refuse(x.device != self.device, "%s is on %s, the plan on %s", name, x.device, self.device)
-        _refuse(tokens is not None and shape[0] != tokens, "%s has %d tokens, wanted %d", name, shape[0], tokens)
-        st = x.stride()
-        _refuse(st[-1] != 1 and shape[-1] > 1, "%s: elements of a head must be contiguous", name)
-        return [0 if n == 1 else s for n, s in zip(shape, st)]           # (the stride of a one-long dimension says nothing)
+    def _rows(self, name, x, heads, dtype, tokens=None):
+        """(token stride, head stride) of x [tokens][heads][head_dim]; refuses what is not such rows of `dtype` on the plan's device."""
+        try:
+            T, h, D = x.shape
+            ld, hs, one = x.stride()
+            if h == heads and D == self.head_dim and x.dtype is dtype and one == 1 and (tokens is None or T == tokens) and x.get_device() == self._index:
+                return 0 if T == 1 else ld, 0 if h == 1 else hs          # (the stride of a one-long dimension says nothing)
+        except (AttributeError, ValueError, TypeError):
+            pass
+        self._not_rows(name, x, heads, dtype, tokens, "[tokens]")
 
-    def _ints(self, name, x, n, dtype=torch.int32):
-        _refuse(not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.dim() != 1 or x.shape[0] != n or x.device != self.device or not x.is_contiguous(),
-                "%s: a contiguous %s tensor of %d values on %s", name, dtype, n, self.device)
+    def _slots(self, name, x, dtype):
+        """(slot stride, row stride, head stride) of a cache x [slots][rows][kv_heads][head_dim]."""
+        try:
+            S, cap, h, D = x.shape
+            ss, ld, hs, one = x.stride()
+            if h == self.kv_heads and D == self.head_dim and x.dtype is dtype and one == 1 and x.get_device() == self._index:
+                return 0 if S == 1 else ss, 0 if cap == 1 else ld, 0 if h == 1 else hs
+        except (AttributeError, ValueError, TypeError):
+            pass
+        self._not_rows(name, x, self.kv_heads, dtype, None, "[slots][rows]")
+
+    def _not_rows(self, name, x, heads, dtype, tokens, lead):
+        _refuse(not isinstance(x, torch.Tensor), "%s is not a tensor", name)
+        _refuse(x.dim() != (3 if lead == "[tokens]" else 4) or x.shape[-2] != heads or x.shape[-1] != self.head_dim, "%s has shape %s, wanted %s[%d][%d]", name,
+                tuple(x.shape), lead, heads, self.head_dim)
+        _refuse(x.dtype is not dtype, "%s is %s, wanted %s", name, x.dtype, dtype)
+        _refuse(x.get_device() != self._index, "%s is on %s, the plan on %s", name, x.device, self.device)
+        _refuse(tokens is not None and x.shape[0] != tokens, "%s has %d tokens, wanted %s", name, x.shape[0], tokens)
+        _refuse(True, "%s: elements of a head must be contiguous", name)
+
+    def _ints(self, name, x, n):
+        """Address of n int32 values on the plan's device."""
+        if not (isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.dim() == 1 and x.shape[0] == n and x.get_device() == self._index
+                and x.is_contiguous()):
+            _refuse(True, "%s: a contiguous int32 tensor of %d values on %s", name, n, self.device)
         return x.data_ptr()
 
     def _launch(self, entry, desc):
-        if self.device.type == "cuda" and torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
-                self.lib.call(entry, C.byref(desc), self._stream())
+        if self._index < 0:
+            self.lib.call(entry, desc, None)
+        elif _current_device() == self._index:
+            self.lib.call(entry, desc, _raw_stream(self._index) if _raw_stream is not None else self._stream().value)
         else:
-            self.lib.call(entry, C.byref(desc), self._stream())
+            with torch.cuda.device(self._index):
+                self.lib.call(entry, desc, self._stream().value)
 
     # ---- rotary positions, norms ---------------------------------------------------------------------------------------------------------
     def rotate(self, q, k, pos, v=None, cache=None, row=None, out=None, inverse=False):
@@ -105,62 +136,64 @@ class AttentionPlan(_Plan):
     def _rotary(self, q, k, pos, v, cache, row, out, inverse, norm):
         _refuse(not self.pairs, "the plan was made without axes")
         H, Hk, D, dt = self.heads, self.kv_heads, self.head_dim, getattr(q, "dtype", None)
-        _refuse(dt not in _DTYPE, "q is %s, wanted float32, float16 or bfloat16", dt)
-        sq = self._rows("q", q, H, dt)
+        if dt not in _DTYPE:
+            _refuse(True, "q is %s, wanted float32, float16 or bfloat16", dt)
+        ldq, hsq = self._rows("q", q, H, dt)
         T = q.shape[0]
-        _refuse(not isinstance(pos, torch.Tensor) or pos.dtype not in (torch.int32, torch.float32) or pos.device != self.device
-                or tuple(pos.shape) != (T, self.naxes) or not pos.is_contiguous(),
-                "pos: a contiguous int32 or float32 tensor [%d][%d] on %s", T, self.naxes, self.device)
-        _refuse(k is None and (v is not None or cache is not None), "v and cache need k")
-        _refuse((cache is None) != (row is None), "cache and row come together")
-        _refuse(cache is None and v is not None, "v needs a cache")
-        d = RotaryDesc()
+        pt = getattr(pos, "dtype", None)
+        if not ((pt is torch.int32 or pt is torch.float32) and pos.shape == (T, self.naxes) and pos.get_device() == self._index and pos.is_contiguous()):
+            _refuse(True, "pos: a contiguous int32 or float32 tensor [%d][%d] on %s", T, self.naxes, self.device)
         q_out, k_out = out if out is not None else (None, None)
         if q_out is None:
-            q_out = torch.empty((T, H, D), dtype=dt, device=self.device)
-        so = self._rows("q_out", q_out, H, dt, T)
-        d.q, d.q_out, d.pos, d.freq, d.axis = q.data_ptr(), q_out.data_ptr(), pos.data_ptr(), self.freq.data_ptr(), self.axis.data_ptr()
-        d.ldq, d.hsq, d.ldqo, d.hsqo = sq[0], sq[1], so[0], so[1]
-        if k is not None:
-            sk = self._rows("k", k, Hk, dt, T)
-            d.k, d.ldk, d.hsk = k.data_ptr(), sk[0], sk[1]
-            if cache is not None:
+            q_out = q.new_empty((T, H, D))
+        ldqo, hsqo = self._rows("q_out", q_out, H, dt, T)
+        kp = vp = kop = vop = rowp = ldk = hsk = ldv = hsv = ldko = hsko = ldvo = hsvo = rows = 0
+        if k is None:
+            _refuse(v is not None or cache is not None or k_out is not None, "v, a cache and out[1] need k")
+        else:
+            ldk, hsk = self._rows("k", k, Hk, dt, T)
+            kp = k.data_ptr()
+            if cache is None:
+                _refuse(row is not None, "cache and row come together")
+                _refuse(v is not None, "v needs a cache")
+                if k_out is None:
+                    k_out = k.new_empty((T, Hk, D))
+                ldko, hsko = self._rows("k_out", k_out, Hk, dt, T)
+            else:
+                _refuse(row is None, "cache and row come together")
                 _refuse(k_out is not None, "out[1] and a cache are one too many")
                 k_out, v_cache = cache
-                rows, d.k_out, d.ldko, d.hsko = self._cache_rows("k_cache", k_out, dt)
-                _refuse((v is None) != (v_cache is None), "v and v_cache come together")
+                rows, ldko, hsko = self._cache_rows("k_cache", k_out, dt)
+                if (v is None) != (v_cache is None):
+                    _refuse(True, "v and v_cache come together")
                 if v is not None:
-                    sv = self._rows("v", v, Hk, dt, T)
-                    d.v, d.ldv, d.hsv = v.data_ptr(), sv[0], sv[1]
-                    vrows, d.v_out, d.ldvo, d.hsvo = self._cache_rows("v_cache", v_cache, dt)
-                    _refuse(vrows != rows, "k_cache has %d rows, v_cache %d", rows, vrows)
-                d.row, d.rows = self._ints("row", row, T), rows
-            else:
-                if k_out is None:
-                    k_out = torch.empty((T, Hk, D), dtype=dt, device=self.device)
-                sk = self._rows("k_out", k_out, Hk, dt, T)
-                d.k_out, d.ldko, d.hsko = k_out.data_ptr(), sk[0], sk[1]
-        d.T, d.Hq, d.Hk, d.D, d.R, d.A = T, H, Hk, D, self.pairs, self.naxes
-        d.dtype, d.pos_float, d.adjacent, d.inverse, d.norm, d.eps = _DTYPE[dt], pos.dtype is torch.float32, self.adjacent, inverse, norm, self.eps
-        if norm:
-            d.q_weight = self.q_weight.data_ptr() if self.q_weight is not None else None
-            d.k_weight = self.k_weight.data_ptr() if self.k_weight is not None else None
+                    ldv, hsv = self._rows("v", v, Hk, dt, T)
+                    vrows, ldvo, hsvo = self._cache_rows("v_cache", v_cache, dt)
+                    if vrows != rows:
+                        _refuse(True, "k_cache has %d rows, v_cache %d", rows, vrows)
+                    vp, vop = v.data_ptr(), v_cache.data_ptr()
+                rowp = self._ints("row", row, T)
+            kop = k_out.data_ptr()
         if T:
-            self._launch("deft_rotary", d)
+            self._launch("deft_rotary", _ROTARY.pack(
+                q.data_ptr(), kp, vp, q_out.data_ptr(), kop, vop, pos.data_ptr(), self._freq_ptr, self._axis_ptr, self._qw_ptr if norm else 0,
+                self._kw_ptr if norm else 0, rowp, ldq, hsq, ldk, hsk, ldv, hsv, ldqo, hsqo, ldko, hsko, ldvo, hsvo, rows,
+                T, H, Hk, D, self.pairs, self.naxes, _DTYPE[dt], pt is torch.float32, self.adjacent, inverse, norm, self.eps))
         return q_out, k_out
 
     def _cache_rows(self, name, x, dt):
-        """(rows, address, row stride, head stride) of a cache [rows][kv_heads][D] or [slots][rows][kv_heads][D] whose slots follow each other."""
-        nd = x.dim() if isinstance(x, torch.Tensor) else 0
-        st = self._rows(name, x, self.kv_heads, dt, ndim=4 if nd == 4 else 3)
-        if nd == 4:
+        """(rows, row stride, head stride) of a cache [rows][kv_heads][D] or [slots][rows][kv_heads][D] whose slots follow each other."""
+        if isinstance(x, torch.Tensor) and x.dim() == 4:
+            ss, ld, hs = self._slots(name, x, dt)
             S, cap = x.shape[0], x.shape[1]
-            _refuse(S > 1 and cap > 1 and st[0] != cap * st[1], "%s: the rows of its slots must follow each other", name)
-            rows, ld = S * cap, st[1] if cap > 1 else st[0]
+            if S > 1 and cap > 1 and ss != cap * ld:
+                _refuse(True, "%s: the rows of its slots must follow each other", name)
+            rows, ld = S * cap, ld if cap > 1 else ss
         else:
-            rows, ld = x.shape[0], st[0]
+            ld, hs = self._rows(name, x, self.kv_heads, dt)
+            rows = x.shape[0]
         _refuse(rows < 1, "%s is empty", name)
-        return rows, x.data_ptr(), ld, st[-2]
+        return rows, ld, hs
 
     # ---- attention -----------------------------------------------------------------------------------------------------------------------
     def attend(self, q, k, v, q_start, k_start=None, slot=None, k_len=None, causal=True, max_k=None, lse=False, out=None):
@@ -171,49 +204,54 @@ class AttentionPlan(_Plan):
         k, v [slots][cap][kv_heads][D]: a cache; its keys are the k_len[b] first rows of slot slot[b].
         causal: query i of n sees the keys j <= m - n + i of its m (a lone new token sees all of them).  Rows that see no key give 0; rows of no
         sequence are not written.  Starts, lengths and slots are int32 device tensors, clamped to the tensors by the kernel; max_k (host): an
-        estimate of the longest m (default: the cap or the number of key rows), which steers only how the work is split.
+        estimate of the longest m, which steers only how the work is split (default: a cache's cap, the number of packed key rows, or twice the
+        average length where keys are the queries' own rows).
         lse=True: returns (o, lse [Tq][heads] float32), the log of each row's sum of exponentials (-inf where it sees no key)."""
         H, Hk, D, dt = self.heads, self.kv_heads, self.head_dim, getattr(q, "dtype", None)
-        _refuse(dt not in _DTYPE, "q is %s, wanted float32, float16 or bfloat16", dt)
-        sq = self._rows("q", q, H, dt)
+        if dt not in _DTYPE:
+            _refuse(True, "q is %s, wanted float32, float16 or bfloat16", dt)
+        ldq, hsq = self._rows("q", q, H, dt)
         Tq = q.shape[0]
-        _refuse(not isinstance(q_start, torch.Tensor) or q_start.dim() != 1 or q_start.shape[0] < 1, "q_start: B + 1 values")
-        B = q_start.shape[0] - 1
-        paged = isinstance(k, torch.Tensor) and k.dim() == 4
-        sk = self._rows("k", k, Hk, dt, ndim=4 if paged else 3)
-        sv = self._rows("v", v, Hk, dt, ndim=4 if paged else 3)
-        _refuse(k.shape != v.shape, "k has shape %s, v %s", tuple(k.shape), tuple(v.shape))
-        d = AttnDesc()
-        d.q_start = self._ints("q_start", q_start, B + 1)
-        if paged:
+        B = q_start.numel() - 1 if isinstance(q_start, torch.Tensor) else -1
+        _refuse(B < 0, "q_start: B + 1 values")
+        qp = self._ints("q_start", q_start, B + 1)
+        cap = ssk = ssv = sp = 0
+        if isinstance(k, torch.Tensor) and k.dim() == 4:
+            ssk, ldk, hsk = self._slots("k", k, dt)
+            ssv, ldv, hsv = self._slots("v", v, dt)
             _refuse(slot is None or k_len is None or k_start is not None, "a cache [slots][cap] needs slot and k_len, and no k_start")
-            d.k_start, d.ssk, d.ssv, d.cap = self._ints("slot", slot, B), sk[0], sv[0], k.shape[1]
-            longest = k.shape[1]
+            sp = self._ints("slot", slot, B)
+            longest = cap = k.shape[1]
         else:
+            ldk, hsk = self._rows("k", k, Hk, dt)
+            ldv, hsv = self._rows("v", v, Hk, dt)
             _refuse(slot is not None, "slot needs a cache [slots][cap][kv_heads][head_dim]")
-            if k_start is not None:
-                d.k_start = self._ints("k_start", k_start, B)
             longest = k.shape[0]
-        if k_len is not None:
-            d.k_len = self._ints("k_len", k_len, B)
+            if k_start is not None:
+                sp = self._ints("k_start", k_start, B)
+            elif k_len is None and B > 1:
+                longest = min(longest, 2 * Tq // B + 1)
+        if k.shape != v.shape:
+            _refuse(True, "k has shape %s, v %s", tuple(k.shape), tuple(v.shape))
+        lp = self._ints("k_len", k_len, B) if k_len is not None else 0
         if out is None:
-            out = torch.empty((Tq, H, D), dtype=dt, device=self.device)
-        so = self._rows("out", out, H, dt, Tq)
+            out = q.new_empty((Tq, H, D))
+            ldo, hso = H * D, D
+        else:
+            ldo, hso = self._rows("out", out, H, dt, Tq)
         logs = torch.empty((Tq, H), dtype=torch.float32, device=self.device) if lse else None
         if Tq and B:
-            empty = not k.numel()                               # nothing to read: every row of a sequence becomes 0
-            d.slots, d.cap = (0, 0) if empty else (k.shape[0], d.cap)
-            if empty:
-                d.k_start = d.k_len = None
-            d.q, d.k, d.v, d.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-            d.lse = logs.data_ptr() if lse else None
-            d.ldq, d.hsq, d.ldk, d.hsk = sq[0], sq[1], sk[-3], sk[-2]
-            d.ldv, d.hsv, d.ldo, d.hso = sv[-3], sv[-2], so[0], so[1]
-            d.Tq, d.B, d.Hq, d.Hk, d.D, d.dtype, d.causal, d.scale = Tq, B, H, Hk, D, _DTYPE[dt], bool(causal), self.scale
-            d.max_k = longest if max_k is None else max(0, min(int(max_k), 0x7fffffff))
-            n = self.lib.value("deft_attn_ws_floats", C.byref(d))
-            if n > 0:
-                ws = torch.empty(n, dtype=torch.float32, device=self.device)       # (stream-ordered: free for the next call once this one is queued)
-                d.ws, d.ws_floats = ws.data_ptr(), n
-            self._launch("deft_attn", d)
+            slots, kp, vp = k.shape[0], k.data_ptr(), v.data_ptr()
+            if not kp or not vp or not k.numel():               # nothing to read: every row of a sequence becomes 0
+                slots = cap = sp = lp = 0
+            if max_k is not None:
+                longest = max(0, min(int(max_k), 0x7fffffff))
+            head = (q.data_ptr(), kp, vp, out.data_ptr(), logs.data_ptr() if lse else 0, qp, sp, lp)
+            tail = (ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso, ssk, ssv, Tq, B, slots, cap, H, Hk, D, _DTYPE[dt], bool(causal), longest, self.scale)
+            ws, n = None, 0
+            if longest > _SPLIT_KEYS:
+                n = self.lib.value("deft_attn_ws_floats", _ATTN.pack(*head, 0, 0, *tail))
+                if n:
+                    ws = torch.empty(n, dtype=torch.float32, device=self.device)   # (stream-ordered: free for the next call once this one is queued)
+            self._launch("deft_attn", _ATTN.pack(*head, ws.data_ptr() if n else 0, n, *tail))
         return (out, logs) if lse else out

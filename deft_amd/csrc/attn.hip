@@ -73,7 +73,7 @@ struct Work {
 };
 
 // Flat tile t -> (sequence, tile of it).  Sequence b starts at flat tile  first(b) = q_start[b] * G / BM + b,  which leaves it at least ceil(n G / BM)
-// tiles whatever the lengths are: no table of lengths is needed on the host, surplus tiles end at once.  64 candidates a step.
+// tiles whatever the lengths are: no table of lengths is needed on the host, surplus tiles end at once.
 template <int BM>
 __device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, unsigned id, int nsplit, int ntiles, Work& w) {
     const int G = p.Hq / p.Hk, lane = threadIdx.x & 63;
@@ -81,18 +81,28 @@ __device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, unsigned
     id /= (unsigned)p.Hk;
     w.split = nsplit == 1 ? 0 : (int)(id % (unsigned)nsplit);
     const int t = ntiles - 1 - (int)(nsplit == 1 ? id : id / (unsigned)nsplit);      // causal: the long rows of a sequence first
+    // the last b with first(b) <= t (first() grows): down to 512 candidates 64 at a time, then 8 loads a lane at once -- one trip to memory, not three
+    auto before = [&](int at) { return clampi(p.q_start[at], 0, p.Tq) * G / BM + at <= t; };      // (Tq * Hq < 2^30)
     int lo = 0, n = p.B;
-    while (true) {
+    while (n > 512) {
         const int step = (n + 63) >> 6, at = lo + lane * step;
-        bool le = false;
-        if (at < lo + n) le = clampi(p.q_start[at], 0, p.Tq) * G / BM + at <= t;      // (Tq * Hq < 2^30)
-        const int c = __popcll(deft_ballot(le));
+        const int c = __popcll(deft_ballot(at < lo + n && before(at)));
         if (c == 0) return false;
         const int left = n - (c - 1) * step;
         lo += (c - 1) * step;
         n = left < step ? left : step;
-        if (n <= 1) break;
     }
+    int c = 0;
+    if (n <= 64) c = __popcll(deft_ballot(lane < n && before(lo + (lane < n ? lane : 0))));
+    else {
+        bool le[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) le[i] = before(lo + (i * 64 + lane < n ? i * 64 + lane : 0));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c += __popcll(deft_ballot(i * 64 + lane < n && le[i]));
+    }
+    if (c == 0) return false;
+    lo += c - 1;
     const int b = w.b = __builtin_amdgcn_readfirstlane(lo);
     w.q0 = clampi(p.q_start[b], 0, p.Tq);
     w.n = clampi(p.q_start[b + 1], 0, p.Tq) - w.q0;
@@ -354,6 +364,37 @@ struct Tile {
 __device__ __forceinline__ size_t ws_row(const DeftAttn& p, int split, int query, int head) { return ((size_t)split * p.Tq + query) * p.Hq + head; }
 __device__ __forceinline__ float* ws_ml(const DeftAttn& p, int nsplit) { return p.ws + (size_t)nsplit * p.Tq * p.Hq * p.D; }
 
+// A wave's 32 rows as they are: to the output, or to the workspace where the keys are split
+template <int DT, int D>
+__device__ __forceinline__ void write_rows(const DeftAttn& p, const Work& w, typename Tile<DT, D>::Rows& rw, int nsplit, int query, int head, bool there, int h) {
+    typedef Tile<DT, D> TL;
+    typedef typename TL::T T;
+    rw.L += __shfl_xor(rw.L, 32);
+    if (!there) return;
+    if (nsplit > 1) {
+        float* const op = p.ws + ws_row(p, w.split, query, head) * D;
+#pragma unroll
+        for (int j = 0; j < TL::NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) *(f32x4*)(op + 32 * j + 2 * r + 4 * h) = f32x4{rw.o[j][r], rw.o[j][r + 1], rw.o[j][r + 2], rw.o[j][r + 3]};
+        if (h == 0) *(float2*)(ws_ml(p, nsplit) + ws_row(p, w.split, query, head) * 2) = make_float2(rw.M, rw.L);
+        return;
+    }
+    const float inv = rw.L == 0.f ? 0.f : 1.f / rw.L;
+    T* const op = (T*)p.o + (long long)query * p.ldo + (long long)head * p.hso;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int j = 0; j < TL::NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            t4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = (T)(rw.o[j][r + e] * inv);
+            *(t4*)(op + 32 * j + 2 * r + 4 * h) = x;
+        }
+    if (p.lse && h == 0) p.lse[(long long)query * p.Hq + head] = rw.L == 0.f ? -INFINITY : (rw.M + deft_log2(rw.L)) * LN2;
+}
+
 constexpr int BM = 128;
 
 template <int DT, int D>
@@ -414,54 +455,19 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, int nsp
             }
         }
     }
-    rw.L += __shfl_xor(rw.L, 32);
-    if (nsplit > 1) {
-        if (row < w.rows) {
-            float* const op = p.ws + ws_row(p, w.split, query, head) * D;
-#pragma unroll
-            for (int j = 0; j < TL::NJ; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) *(f32x4*)(op + 32 * j + 2 * r + 4 * h) = f32x4{rw.o[j][r], rw.o[j][r + 1], rw.o[j][r + 2], rw.o[j][r + 3]};
-            if (h == 0) {
-                float* const ml = ws_ml(p, nsplit) + ws_row(p, w.split, query, head) * 2;
-                ml[0] = rw.M;
-                ml[1] = rw.L;
-            }
-        }
-        return;
-    }
-    const float inv = rw.L == 0.f ? 0.f : 1.f / rw.L;
-    if (row < w.rows) {
-        T* const op = (T*)p.o + (long long)query * p.ldo + (long long)head * p.hso;
-        typedef T t4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-        for (int j = 0; j < TL::NJ; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                t4 x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = (T)(rw.o[j][r + e] * inv);
-                *(t4*)(op + 32 * j + 2 * r + 4 * h) = x;
-            }
-        if (p.lse && h == 0) p.lse[(long long)query * p.Hq + head] = rw.L == 0.f ? -INFINITY : (rw.M + deft_log2(rw.L)) * LN2;
-    }
+    write_rows<DT, D>(p, w, rw, nsplit, query, head, row < w.rows, h);
 }
 
-template <int DT, int D>
-struct StepCfg {
-    typedef Tile<DT, D> TL;
-    static constexpr int NW = TL::RB > 256 ? 2 : 4;               // waves: two 32-key stages of K and V each stay within 128 KB
-    static constexpr int KB = 32 * TL::RB, LDS = NW * 4 * KB;
-};
+// waves that share the keys of a row tile: two 32-key stages of K and V each stay within 128 KB
+template <int DT, int D> constexpr int step_waves() { return Tile<DT, D>::RB > 256 ? 2 : 4; }
 
-template <int DT, int D>
-__global__ __launch_bounds__(64 * (StepCfg<DT, D>::NW)) void attn_step_kernel(DeftAttn p, int nsplit, int ntiles) {
+template <int DT, int D, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(DeftAttn p, int nsplit, int ntiles) {
     typedef Tile<DT, D> TL;
     typedef typename TL::T T;
-    typedef StepCfg<DT, D> C;
-    constexpr int NW = C::NW, KB = C::KB, NI = TL::CPR / 2;
-    static_assert(C::LDS >= NW * 32 * D * 4, "the join fits the stages");
-    __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+    constexpr int KB = 32 * TL::RB, LDS = NW * 4 * KB, NI = TL::CPR / 2;
+    static_assert(LDS >= NW * 32 * D * 4, "the join fits the stages");
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];
     __shared__ float ms[NW][32], ls[NW][32];
     const int G = p.Hq / p.Hk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
     Work w;
@@ -509,6 +515,10 @@ __global__ __launch_bounds__(64 * (StepCfg<DT, D>::NW)) void attn_step_kernel(De
             TL::template step<1, true>(rw, mine, mine + KB, vis - t * 32, true, false, sc, lane);
         }
     }
+    if constexpr (NW == 1) {
+        write_rows<DT, D>(p, w, rw, nsplit, query, head, row <= last, h);
+        return;
+    }
     // join the waves: everybody's M and L, then O scaled to the common M, summed in wave order
     rw.L += __shfl_xor(rw.L, 32);
     if (h == 0) { ms[wave][l32] = rw.M; ls[wave][l32] = rw.L; }
@@ -541,11 +551,7 @@ __global__ __launch_bounds__(64 * (StepCfg<DT, D>::NW)) void attn_step_kernel(De
         const int qr = w.q0 + (w.row0 + r) / G, hd = w.hk * G + (w.row0 + r) % G;
         if (nsplit > 1) {
             *(f32x4*)(p.ws + ws_row(p, w.split, qr, hd) * D + c) = x;
-            if (c == 0) {
-                float* const ml = ws_ml(p, nsplit) + ws_row(p, w.split, qr, hd) * 2;
-                ml[0] = Mr;
-                ml[1] = Lr;
-            }
+            if (c == 0) *(float2*)(ws_ml(p, nsplit) + ws_row(p, w.split, qr, hd) * 2) = make_float2(Mr, Lr);
         } else {
             const float inv = Lr == 0.f ? 0.f : 1.f / Lr;
             typedef T t4 __attribute__((ext_vector_type(4)));
@@ -566,20 +572,20 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(DeftAttn p, int nsplit)
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int q = (int)(row / p.Hq), h = (int)(row - (long long)q * p.Hq);
     if (q >= p.Tq || q < p.q_start[0] || q >= p.q_start[p.B]) return;
-    const float* const ml = ws_ml(p, nsplit);
-    float M = M_NONE;
-    for (int s = 0; s < nsplit; ++s) M = fmaxf(M, ml[ws_row(p, s, q, h) * 2]);
-    float L = 0.f, o0 = 0.f, o1 = 0.f;
+    // lane s: M and L of split s (at most 64); then the splits' rows, whose loads wait for nothing
+    const float2 x = lane < nsplit ? *(const float2*)(ws_ml(p, nsplit) + ws_row(p, lane, q, h) * 2) : make_float2(M_NONE, 0.f);
+    float M = x.x;
+    for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i));
+    const float al = deft_exp2(x.x - M);
+    float L = x.y * al, o0 = 0.f, o1 = 0.f;
+    for (int i = 1; i < 64; i <<= 1) L += __shfl_xor(L, i);
+    const int col = lane * 2 < p.D ? lane * 2 : 0;
+#pragma unroll 4
     for (int s = 0; s < nsplit; ++s) {
-        const size_t at = ws_row(p, s, q, h);
-        const float al = deft_exp2(ml[at * 2] - M), l = ml[at * 2 + 1];
-        if (l == 0.f) continue;                                    // saw no key
-        L = fmaf(l, al, L);
-        if (lane * 2 < p.D) {
-            const float2 x = *(const float2*)(p.ws + at * p.D + lane * 2);
-            o0 = fmaf(x.x, al, o0);
-            o1 = fmaf(x.y, al, o1);
-        }
+        const float2 y = *(const float2*)(p.ws + ws_row(p, s, q, h) * p.D + col);
+        const float a = __shfl(al, s);
+        o0 = fmaf(y.x, a, o0);
+        o1 = fmaf(y.y, a, o1);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     if (lane * 2 < p.D) {
@@ -612,13 +618,14 @@ int attn_check(const DeftAttn* d) {
 }
 
 // How a call runs: the kernel, its flat tiles, and over how many workgroups the keys of a tile are split.
-struct Choice { bool step; int nsplit, ntiles; };
+struct Choice { bool step; int waves, nsplit, ntiles; };
 Choice choose(const DeftAttn* d) {
     const int G = d->Hq / d->Hk;
     Choice c;
     c.step = (long long)d->Tq * G <= 32ll * d->B;                  // up to 32 rows a sequence on average
     const int bm = c.step ? 32 : BM;
     c.ntiles = d->Tq * G / bm + d->B;                              // (below 2^26 + 2^24)
+    c.waves = !c.step ? 4 : d->max_k <= 64 ? 1 : d->dtype == DEFT_F32 && d->D > 64 ? 2 : 4;
     // rows that are there fill about this many workgroups
     const long long busy = ((long long)d->Tq * G / bm + (c.step ? d->B : d->B / 2 + 1)) * d->Hk;
     const int keys = c.step ? 256 : 512;                           // keys a split should have at least
@@ -632,8 +639,10 @@ Choice choose(const DeftAttn* d) {
 
 template <int DT, int D>
 void attn_launch(const DeftAttn& d, const Choice& c, unsigned grid, hipStream_t s) {
-    if (c.step) hipLaunchKernelGGL((attn_step_kernel<DT, D>), dim3(grid), dim3(64 * StepCfg<DT, D>::NW), 0, s, d, c.nsplit, c.ntiles);
-    else hipLaunchKernelGGL((attn_prompt_kernel<DT, D>), dim3(grid), dim3(256), 0, s, d, c.nsplit, c.ntiles);
+    constexpr int NW = step_waves<DT, D>();
+    if (!c.step) hipLaunchKernelGGL((attn_prompt_kernel<DT, D>), dim3(grid), dim3(256), 0, s, d, c.nsplit, c.ntiles);
+    else if (c.waves == 1) hipLaunchKernelGGL((attn_step_kernel<DT, D, 1>), dim3(grid), dim3(64), 0, s, d, c.nsplit, c.ntiles);
+    else hipLaunchKernelGGL((attn_step_kernel<DT, D, NW>), dim3(grid), dim3(64 * NW), 0, s, d, c.nsplit, c.ntiles);
 }
 template <int DT>
 void attn_launch_d(const DeftAttn& d, const Choice& c, unsigned grid, hipStream_t s) {

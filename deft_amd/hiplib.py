@@ -95,9 +95,9 @@ _SIGS = {
     "deft_conv_direct": (C.c_int, [C.POINTER(GemmDesc), c_fp]),
     "deft_split_weights_direct": (C.c_int, [c_fp, c_fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, c_fp]),
     "deft_direct_weight_bytes": (C.c_longlong, [C.c_int, C.c_int, C.c_int, C.c_int]),
-    "deft_rotary": (C.c_int, [C.POINTER(RotaryDesc), c_fp]),
-    "deft_attn": (C.c_int, [C.POINTER(AttnDesc), c_fp]),
-    "deft_attn_ws_floats": (C.c_longlong, [C.POINTER(AttnDesc)]),
+    "deft_rotary": (C.c_int, [c_fp, c_fp]),               # DeftRotary / DeftAttn: a RotaryDesc / AttnDesc by reference, or its packed bytes
+    "deft_attn": (C.c_int, [c_fp, c_fp]),
+    "deft_attn_ws_floats": (C.c_longlong, [c_fp]),
     "deft_track_similarity": (C.c_int, [c_fp] + [C.c_int] * 2 + [c_fp] * 3 + [C.c_int] * 2 + [c_fp, c_fp]),
     # host-side association helpers (HOST pointers, synchronous)
     "deft_lapjv": (C.c_int, [c_fp, C.c_int, C.c_int, C.c_double, c_fp, c_fp, c_fp]),

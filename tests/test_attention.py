@@ -164,3 +164,12 @@ def test_descriptor_layouts_match_the_header():
         for decl in re.findall(r"(?:const void|const double|const int|const float|void|float|long long|int)\s*([^;]+);", body):
             names += [n.strip().lstrip("* ") for n in decl.split(",")]
         assert names == [n for n, _ in mirror._fields_]
+
+
+def test_packed_descriptors_match_the_mirrors():
+    """The struct formats that deft_amd.attention packs are the ctypes layouts: same size, same place for every field."""
+    from deft_amd import attention, hiplib
+    for fmt, mirror in ((attention._ROTARY, hiplib.RotaryDesc), (attention._ATTN, hiplib.AttnDesc)):
+        vals = [i + 1 for i in range(len(mirror._fields_) - 1)] + [0.5]
+        d = mirror.from_buffer_copy(fmt.pack(*vals))
+        assert [getattr(d, n) for n, _ in mirror._fields_] == vals
