@@ -32,24 +32,67 @@ __device__ __forceinline__ void turn_sincos(double r, float& sn, float& cs) {
     cs = ((quad + 1) & 2) ? -b : b;
 }
 
+#ifndef DEFT_DPP_HOOK          /* the unit-test SIMT emulator pre-defines these hooks */
+#define DEFT_DPP_XCHG(v, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true))
+// v + the value of lane l ^ S, where the lanes of each aligned group of S hold the same v: exchanges inside the register file (S < 16) -- quad
+// permutations, then mirrors of 8 and 16 lanes, which meet a lane of the other half
+template <int S> __device__ __forceinline__ float deft_add_xor(float v) {
+    if constexpr (S == 1) return v + DEFT_DPP_XCHG(v, 0xB1);
+    else if constexpr (S == 2) return v + DEFT_DPP_XCHG(v, 0x4E);
+    else if constexpr (S == 4) return v + DEFT_DPP_XCHG(v, 0x141);
+    else if constexpr (S == 8) return v + DEFT_DPP_XCHG(v, 0x140);
+    else return v + __shfl_xor(v, S);
+}
+__device__ __forceinline__ float deft_rsq(float x) { return __builtin_amdgcn_rsqf(x); }
+#endif
+
 // One wave: one token, `parts` waves sharing its heads.  LPH lanes a head (a power of two >= D / 2V; the surplus lanes of D = 96 idle).
-template <int DT, bool ADJ>
-__global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, int lph_log2, int parts) {
+// The heads of the next pass are fetched before those of this one are worked on, the first ones before the angles; norm weights stay in registers.
+template <int DT, bool ADJ, bool NORM, int LPH>
+__global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, int parts, float inv_d) {
     typedef typename Elem<DT>::T T;
-    constexpr int V = 16 / (int)sizeof(T);
+    constexpr int V = 16 / (int)sizeof(T), HPW = 64 / LPH;
     typedef T vec __attribute__((ext_vector_type(V)));
     __shared__ __attribute__((aligned(16))) float cs_s[ROT_WAVES][2][ROT_MAX_PAIRS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long unit = (long long)blockIdx.x * ROT_WAVES + wave;
-    const int t = (int)(unit / parts), part = (int)(unit - (long long)t * parts);
+    const unsigned unit = blockIdx.x * ROT_WAVES + wave;                           // (T * parts < 2^31)
+    const int t = __builtin_amdgcn_readfirstlane((int)(parts == 1 ? unit : unit / (unsigned)parts)), part = __builtin_amdgcn_readfirstlane((int)(unit - (unsigned)t * (unsigned)parts));
     const bool live = t < p.T;
+    const int c = lane & (LPH - 1), sub = lane / LPH;
+    const bool mine = live && c < p.D / (2 * V);
+    const bool turns = c * V < p.R;
+    // this lane's two chunks; the pairs whose sines and cosines it needs are c V .. c V + V - 1
+    const int lo = ADJ || !turns ? c * 2 * V : c * V;
+    const int hi = ADJ || !turns ? lo + V : p.R + c * V;
+    const int Hqk = p.Hq + (p.k ? p.Hk : 0), Hall = Hqk + (p.v ? p.Hk : 0);
+    long long krow = t;
+    bool kput = true;
+    if (live && p.row && p.k) {
+        krow = p.row[t];
+        kput = krow >= 0 && krow < p.rows;
+    }
+    const T* const qt = (const T*)p.q + (long long)t * p.ldq;
+    const T* const kt = (const T*)p.k + (long long)t * p.ldk;
+    const T* const vt = (const T*)p.v + (long long)t * p.ldv;
+    auto load = [&](int h, vec& a, vec& b) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { a[e] = (T)0.f; b[e] = (T)0.f; }
+        if (mine && h < Hall) {
+            const T* src = h < p.Hq ? qt + (long long)h * p.hsq : h < Hqk ? kt + (long long)(h - p.Hq) * p.hsk : vt + (long long)(h - Hqk) * p.hsv;
+            a = *(const vec*)(src + lo);
+            b = *(const vec*)(src + hi);
+        }
+    };
+    int h = part * HPW + sub;
+    vec a, b;
+    load(h, a, b);
     float* const cs_c = cs_s[wave][0];
     float* const cs_n = cs_s[wave][1];
     if (live) {
         for (int i = lane; i < p.R; i += 64) {
-            int a = p.axis[i];
-            a = a < 0 ? 0 : (a < p.A ? a : p.A - 1);
-            const size_t at = (size_t)t * p.A + a;
+            int ax = p.axis[i];
+            ax = ax < 0 ? 0 : (ax < p.A ? ax : p.A - 1);
+            const size_t at = (size_t)t * p.A + ax;
             const double x = p.pos_float ? (double)((const float*)p.pos)[at] : (double)((const int*)p.pos)[at];
             float sn, cs;
             turn_sincos(x * p.freq[i] * 0.15915494309189535, sn, cs);
@@ -59,88 +102,74 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
     }
     __syncthreads();
     if (!live) return;
-    const int lph = 1 << lph_log2, hpw = 64 >> lph_log2;
-    const int c = lane & (lph - 1), sub = lane >> lph_log2;
-    const bool mine = c < p.D / (2 * V);
-    const bool turns = c * V < p.R;
-    // this lane's two chunks, and the sines and cosines of the pairs c V .. c V + V - 1
-    const int lo = ADJ || !turns ? c * 2 * V : c * V;
-    const int hi = ADJ || !turns ? lo + V : p.R + c * V;
-    float cv[V], sv[V];
+    float cv[V], sv[V], wq[2 * V], wk[2 * V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         cv[e] = turns ? cs_c[c * V + e] : 1.f;
         sv[e] = turns ? cs_n[c * V + e] : 0.f;
     }
-    const int Hqk = p.Hq + (p.k ? p.Hk : 0), Hall = Hqk + (p.v ? p.Hk : 0);
-    long long krow = t;
-    bool kput = true;
-    if (p.row && p.k) {
-        krow = p.row[t];
-        kput = krow >= 0 && krow < p.rows;
-    }
-    for (int h0 = part * hpw; h0 < Hall; h0 += parts * hpw) {
-        const int h = h0 + sub;
-        const bool isq = h < p.Hq, isv = h >= Hqk;
-        const bool on = mine && h < Hall;
-        const T* src = nullptr;
-        T* dst = nullptr;
-        if (on) {
-            if (isq) {
-                src = (const T*)p.q + (long long)t * p.ldq + (long long)h * p.hsq;
-                dst = (T*)p.q_out + (long long)t * p.ldqo + (long long)h * p.hsqo;
-            } else if (!isv) {
-                src = (const T*)p.k + (long long)t * p.ldk + (long long)(h - p.Hq) * p.hsk;
-                dst = (T*)p.k_out + krow * p.ldko + (long long)(h - p.Hq) * p.hsko;
-            } else {
-                src = (const T*)p.v + (long long)t * p.ldv + (long long)(h - Hqk) * p.hsv;
-                dst = (T*)p.v_out + krow * p.ldvo + (long long)(h - Hqk) * p.hsvo;
-            }
-        }
-        vec a, b;
+    if constexpr (NORM) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) { a[e] = (T)0.f; b[e] = (T)0.f; }
-        if (on) { a = *(const vec*)(src + lo); b = *(const vec*)(src + hi); }
+        for (int e = 0; e < 2 * V; ++e) {
+            const int d = e < V ? lo + e : hi + e - V;
+            wq[e] = p.q_weight && mine ? p.q_weight[d] : 1.f;
+            wk[e] = p.k_weight && mine ? p.k_weight[d] : 1.f;
+        }
+    }
+    for (int h0 = part * HPW; h0 < Hall; h0 += parts * HPW) {
+        vec a2, b2;
+        load(h + parts * HPW, a2, b2);
+        const bool isq = h < p.Hq, isv = h >= Hqk;
         float x[V], y[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) { x[e] = (float)a[e]; y[e] = (float)b[e]; }
-        if (p.norm) {
+        if constexpr (NORM) {
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < V; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
-            for (int s = 1; s < lph; s <<= 1) ss += __shfl_xor(ss, s);
-            const float r = 1.f / sqrtf(ss / (float)p.D + p.eps);
-            const float* w = isq ? p.q_weight : p.k_weight;
+            if constexpr (LPH > 1) ss = deft_add_xor<1>(ss);
+            if constexpr (LPH > 2) ss = deft_add_xor<2>(ss);
+            if constexpr (LPH > 4) ss = deft_add_xor<4>(ss);
+            if constexpr (LPH > 8) ss = deft_add_xor<8>(ss);
+            if constexpr (LPH > 16) ss = deft_add_xor<16>(ss);
+            const float m = fmaf(ss, inv_d, p.eps);
+            const float r = m >= 1e-30f ? deft_rsq(m) : 1.f / sqrtf(m);            // (the hardware's root takes no subnormal)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                x[e] *= r * (w && on ? w[lo + e] : 1.f);
-                y[e] *= r * (w && on ? w[hi + e] : 1.f);
+                x[e] *= r * (isq ? wq[e] : wk[e]);
+                y[e] *= r * (isq ? wq[V + e] : wk[V + e]);
             }
         }
-        if (!on || !(isq || kput)) continue;
-        if (!isv) {
-            if (ADJ) {
+        if (mine && h < Hall && (isq || kput)) {
+            if (!isv) {
+                if constexpr (ADJ) {
 #pragma unroll
-                for (int e = 0; e < V; e += 2) {
-                    const float x0 = x[e], x1 = x[e + 1], y0 = y[e], y1 = y[e + 1];
-                    x[e] = x0 * cv[e / 2] - x1 * sv[e / 2];
-                    x[e + 1] = x1 * cv[e / 2] + x0 * sv[e / 2];
-                    y[e] = y0 * cv[V / 2 + e / 2] - y1 * sv[V / 2 + e / 2];
-                    y[e + 1] = y1 * cv[V / 2 + e / 2] + y0 * sv[V / 2 + e / 2];
-                }
-            } else {
+                    for (int e = 0; e < V; e += 2) {
+                        const float x0 = x[e], x1 = x[e + 1], y0 = y[e], y1 = y[e + 1];
+                        x[e] = x0 * cv[e / 2] - x1 * sv[e / 2];
+                        x[e + 1] = x1 * cv[e / 2] + x0 * sv[e / 2];
+                        y[e] = y0 * cv[V / 2 + e / 2] - y1 * sv[V / 2 + e / 2];
+                        y[e + 1] = y1 * cv[V / 2 + e / 2] + y0 * sv[V / 2 + e / 2];
+                    }
+                } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float xe = x[e], ye = y[e];
-                    x[e] = xe * cv[e] - ye * sv[e];
-                    y[e] = ye * cv[e] + xe * sv[e];
+                    for (int e = 0; e < V; ++e) {
+                        const float xe = x[e], ye = y[e];
+                        x[e] = xe * cv[e] - ye * sv[e];
+                        y[e] = ye * cv[e] + xe * sv[e];
+                    }
                 }
+#pragma unroll
+                for (int e = 0; e < V; ++e) { a[e] = (T)x[e]; b[e] = (T)y[e]; }
             }
-#pragma unroll
-            for (int e = 0; e < V; ++e) { a[e] = (T)x[e]; b[e] = (T)y[e]; }
+            T* const dst = isq ? (T*)p.q_out + (long long)t * p.ldqo + (long long)h * p.hsqo
+                               : !isv ? (T*)p.k_out + krow * p.ldko + (long long)(h - p.Hq) * p.hsko : (T*)p.v_out + krow * p.ldvo + (long long)(h - Hqk) * p.hsvo;
+            *(vec*)(dst + lo) = a;
+            *(vec*)(dst + hi) = b;
         }
-        *(vec*)(dst + lo) = a;
-        *(vec*)(dst + hi) = b;
+        a = a2;
+        b = b2;
+        h += parts * HPW;
     }
 }
 
@@ -150,10 +179,28 @@ bool out_fits(long long ld, long long hs, int V, long long rows, int H, int D) {
     return in_fits(ld, hs, V) && (rows <= 1 || ld >= D) && (H <= 1 || hs >= D);
 }
 
+struct RotLaunch { unsigned grid; int parts; float inv_d; hipStream_t s; };
+template <int DT, int LPH>
+void rotary_launch(const DeftRotary& d, const RotLaunch& l) {
+    const dim3 g(l.grid), b(64 * ROT_WAVES);
+    if (d.norm) {
+        if (d.adjacent) hipLaunchKernelGGL((rotary_kernel<DT, true, true, LPH>), g, b, 0, l.s, d, l.parts, l.inv_d);
+        else hipLaunchKernelGGL((rotary_kernel<DT, false, true, LPH>), g, b, 0, l.s, d, l.parts, l.inv_d);
+    } else {
+        if (d.adjacent) hipLaunchKernelGGL((rotary_kernel<DT, true, false, LPH>), g, b, 0, l.s, d, l.parts, l.inv_d);
+        else hipLaunchKernelGGL((rotary_kernel<DT, false, false, LPH>), g, b, 0, l.s, d, l.parts, l.inv_d);
+    }
+}
 template <int DT>
-void rotary_launch(const DeftRotary& d, hipStream_t s, int lph_log2, int parts, unsigned grid) {
-    if (d.adjacent) hipLaunchKernelGGL((rotary_kernel<DT, true>), dim3(grid), dim3(64 * ROT_WAVES), 0, s, d, lph_log2, parts);
-    else hipLaunchKernelGGL((rotary_kernel<DT, false>), dim3(grid), dim3(64 * ROT_WAVES), 0, s, d, lph_log2, parts);
+void rotary_launch_lanes(const DeftRotary& d, const RotLaunch& l, int lanes) {
+    switch (lanes) {
+        case 1: rotary_launch<DT, 1>(d, l); break;
+        case 2: rotary_launch<DT, 2>(d, l); break;
+        case 4: rotary_launch<DT, 4>(d, l); break;
+        case 8: rotary_launch<DT, 8>(d, l); break;
+        case 16: rotary_launch<DT, 16>(d, l); break;
+        default: if constexpr (DT == DEFT_F32) rotary_launch<DT, 32>(d, l);         // (fp32, D > 128)
+    }
 }
 
 }  // namespace
@@ -184,19 +231,19 @@ extern "C" int deft_rotary(const DeftRotary* d, void* stream) {
     DEFT_CHECK(fit, -125, "deft_rotary: strides must be multiples of %d elements and keep heads apart", V);
     DEFT_CHECK(!d->row || d->rows >= 0, -126, "deft_rotary: rows=%lld", d->rows);
     if (d->T == 0) return 0;
-    int lph_log2 = 0;
-    while ((1 << lph_log2) < d->D / (2 * V)) ++lph_log2;
+    int lanes = 1;
+    while (lanes < d->D / (2 * V)) lanes *= 2;
     const int heads = d->Hq + (d->k ? d->Hk : 0) + (d->v ? d->Hk : 0);
-    const int passes = deft_cdiv(heads, 64 >> lph_log2);
+    const int passes = deft_cdiv(heads, 64 / lanes);
     // waves per token: one is the least angle work; few tokens take more, up to one pass each, until the chip's 256 x 16 waves are there
     int parts = 1;
     while (parts < passes && (long long)d->T * parts < 4096) ++parts;
     const long long units = (long long)d->T * parts;
-    const unsigned grid = (unsigned)((units + ROT_WAVES - 1) / ROT_WAVES);
-    hipStream_t s = (hipStream_t)stream;
-    if (d->dtype == DEFT_F32) rotary_launch<DEFT_F32>(*d, s, lph_log2, parts, grid);
-    else if (d->dtype == DEFT_F16) rotary_launch<DEFT_F16>(*d, s, lph_log2, parts, grid);
-    else rotary_launch<DEFT_BF16>(*d, s, lph_log2, parts, grid);
+    DEFT_CHECK(units < (1ll << 31), -123, "deft_rotary: T=%d", d->T);
+    const RotLaunch l = {(unsigned)((units + ROT_WAVES - 1) / ROT_WAVES), parts, 1.f / (float)d->D, (hipStream_t)stream};
+    if (d->dtype == DEFT_F32) rotary_launch_lanes<DEFT_F32>(*d, l, lanes);
+    else if (d->dtype == DEFT_F16) rotary_launch_lanes<DEFT_F16>(*d, l, lanes);
+    else rotary_launch_lanes<DEFT_BF16>(*d, l, lanes);
     DEFT_CHECK_LAUNCH("rotary");
     return 0;
 }

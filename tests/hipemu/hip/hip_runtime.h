@@ -532,6 +532,10 @@ static inline unsigned long long deft_ballot(bool b) {
     for (int l = 0; l < 64; ++l) m |= (unsigned long long)(A[l] != 0.f) << l;
     return m;
 }
+// hooks of deft_amd/csrc/rotary.hip
+#define DEFT_DPP_HOOK 1
+template <int S> static inline float deft_add_xor(float v) { return v + __shfl_xor(v, S); }
+static inline float deft_rsq(float x) { return 1.f / sqrtf(x); }
 static inline float deft_exp2(float x) { return exp2f(x); }
 static inline float deft_log2(float x) { return log2f(x); }
 static inline int __popcll(unsigned long long x) { return __builtin_popcountll(x); }
