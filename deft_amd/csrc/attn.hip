@@ -360,28 +360,47 @@ struct Tile {
     }
 };
 
+// Key tiles (of bn keys) a split takes: a fixed piece, 1 / nsplit of the longest sequence, so that the workgroups of long and short sequences take
+// equally long (a short one's later splits have nothing to do); more where max_k was too low an estimate.
+__device__ __forceinline__ int split_tiles(const DeftAttn& p, int nt, int bn, int nsplit) {
+    const int even = (nt + nsplit - 1) / nsplit, fixed = nsplit == 1 ? even : ((p.max_k + bn - 1) / bn + nsplit - 1) / nsplit;
+    return even > fixed ? even : fixed;
+}
+
 // Where a split's partial results stand in the workspace: O [split][row][D], then (M, L) [split][row]; row = query * Hq + head
 __device__ __forceinline__ size_t ws_row(const DeftAttn& p, int split, int query, int head) { return ((size_t)split * p.Tq + query) * p.Hq + head; }
 __device__ __forceinline__ float* ws_ml(const DeftAttn& p, int nsplit) { return p.ws + (size_t)nsplit * p.Tq * p.Hq * p.D; }
 
-// A wave's 32 rows as they are: to the output, or to the workspace where the keys are split
+// A wave's 32 rows to the output, or to the workspace where the keys are split: through its part of the LDS stages (32 rows, chunks swizzled like
+// K's), so that rows leave as whole lines -- in the accumulators a lane holds 4 of every 8 columns of one row.
 template <int DT, int D>
-__device__ __forceinline__ void write_rows(const DeftAttn& p, const Work& w, typename Tile<DT, D>::Rows& rw, int nsplit, int query, int head, bool there, int h) {
+__device__ __forceinline__ void write_rows(const DeftAttn& p, const Work& w, typename Tile<DT, D>::Rows& rw, int nsplit, int query, int head, int nrows, int lane, char* part) {
     typedef Tile<DT, D> TL;
     typedef typename TL::T T;
+    const int h = lane >> 5, l32 = lane & 31;
     rw.L += __shfl_xor(rw.L, 32);
-    if (!there) return;
+    const bool there = l32 < nrows;
+    const int at = query * p.Hq + head;                                            // (Tq * Hq < 2^30)
     if (nsplit > 1) {
-        float* const op = p.ws + ws_row(p, w.split, query, head) * D;
+        typedef Tile<DEFT_F32, D> TF;
+        if (h == 0 && there) *(float2*)(ws_ml(p, nsplit) + ((size_t)w.split * p.Tq * p.Hq + at) * 2) = make_float2(rw.M, rw.L);
+        if (deft_ballot(rw.L != 0.f) == 0) return;                                 // (no row saw a key of this split: nobody reads its O)
 #pragma unroll
-        for (int j = 0; j < TL::NJ; ++j)
+        for (int j = 0; j < TF::NJ; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) *(f32x4*)(op + 32 * j + 2 * r + 4 * h) = f32x4{rw.o[j][r], rw.o[j][r + 1], rw.o[j][r + 2], rw.o[j][r + 3]};
-        if (h == 0) *(float2*)(ws_ml(p, nsplit) + ws_row(p, w.split, query, head) * 2) = make_float2(rw.M, rw.L);
+            for (int r = 0; r < 16; r += 4)
+                *(f32x4*)(part + l32 * TF::RB + (((8 * j + r / 2 + h) ^ TF::fk(l32)) << 4)) = f32x4{rw.o[j][r], rw.o[j][r + 1], rw.o[j][r + 2], rw.o[j][r + 3]};
+        DEFT_WAVE_LGKM();
+#pragma unroll
+        for (int i = 0; i < TF::CPR / 2; ++i) {
+            const int s = i * 64 + lane, r = s / TF::CPR, c = s - r * TF::CPR;
+            const f32x4 x = *(const f32x4*)(part + r * TF::RB + ((c ^ TF::fk(r)) << 4));
+            const int ar = __shfl(at, r);
+            if (r < nrows) *(f32x4*)(p.ws + ((size_t)w.split * p.Tq * p.Hq + ar) * D + c * 4) = x;
+        }
         return;
     }
     const float inv = rw.L == 0.f ? 0.f : 1.f / rw.L;
-    T* const op = (T*)p.o + (long long)query * p.ldo + (long long)head * p.hso;
     typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int j = 0; j < TL::NJ; ++j)
@@ -390,9 +409,18 @@ __device__ __forceinline__ void write_rows(const DeftAttn& p, const Work& w, typ
             t4 x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = (T)(rw.o[j][r + e] * inv);
-            *(t4*)(op + 32 * j + 2 * r + 4 * h) = x;
+            const int byte = (32 * j + 2 * r + 4 * h) * TL::TS;
+            *(t4*)(part + l32 * TL::RB + (((byte >> 4) ^ TL::fk(l32)) << 4) + (byte & 15)) = x;
         }
-    if (p.lse && h == 0) p.lse[(long long)query * p.Hq + head] = rw.L == 0.f ? -INFINITY : (rw.M + deft_log2(rw.L)) * LN2;
+    DEFT_WAVE_LGKM();
+    if (p.lse && h == 0 && there) p.lse[at] = rw.L == 0.f ? -INFINITY : (rw.M + deft_log2(rw.L)) * LN2;
+#pragma unroll
+    for (int i = 0; i < TL::CPR / 2; ++i) {
+        const int s = i * 64 + lane, r = s / TL::CPR, c = s - r * TL::CPR;
+        const u32x4 x = *(const u32x4*)(part + r * TL::RB + ((c ^ TL::fk(r)) << 4));
+        const int qr = __shfl(query, r), hr = __shfl(head, r);
+        if (r < nrows) *(u32x4*)((char*)p.o + ((long long)qr * p.ldo + (long long)hr * p.hso) * TL::TS + c * 16) = x;
+    }
 }
 
 constexpr int BM = 128;
@@ -417,11 +445,9 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, int nsp
     const int vmin = __builtin_amdgcn_readfirstlane(visible(p, w, wr0 < last ? wr0 : last, G));               // the wave's first and last row
     const int vmax = __builtin_amdgcn_readfirstlane(visible(p, w, wr0 + 31 < last ? wr0 + 31 : last, G));
     const int bmax = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0 + BM - 1 < last ? w.row0 + BM - 1 : last, G));
-    const int nt = (bmax + BN - 1) / BN, per = (nt + nsplit - 1) / nsplit;
+    const int nt = (bmax + BN - 1) / BN, per = split_tiles(p, nt, BN, nsplit);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
-    typename TL::Rows rw;
-    rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
     typename TL::template Fetch<NI> fk, fv;
     fk.init(lane, wave, 4, p.ldk, [](int r) { return TL::fk(r); });
     fv.init(lane, wave, 4, p.ldv, [](int r) { return TL::fv(r); });
@@ -434,6 +460,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, int nsp
     };
     if (tid == 0) again = 0;
     if (t0 < t1) issue(t0);
+    typename TL::Rows rw;                                                          // (its loads and the first tile's are one trip to memory)
+    rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
     for (int t = t0; t < t1; ++t) {
         DEFT_PIPE_BARRIER(0);                                                      // tile t is here, and nobody reads tile t - 1 any more
         if (t + 1 < t1) issue(t + 1);
@@ -453,9 +481,11 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, int nsp
                 DEFT_PIPE_BARRIER(0);
                 if (on && t * BN < vmax) TL::template step<NT, true>(rw, lds + (t & 1) * KB, lds + 2 * KB + (t & 1) * KB, vis - t * BN, true, false, sc, lane);
             }
+            __syncthreads();
         }
     }
-    write_rows<DT, D>(p, w, rw, nsplit, query, head, row < w.rows, h);
+    if (!p.causal) __syncthreads();                                                // (nobody reads the stages any more)
+    write_rows<DT, D>(p, w, rw, nsplit, query, head, w.rows - wr0, lane, lds + wave * KB);
 }
 
 // waves that share the keys of a row tile: two 32-key stages of K and V each stay within 128 KB
@@ -478,11 +508,9 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
     const int vis = visible(p, w, rc, G);
     const int vmin = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0, G));
     const int vmax = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0 + 31 < last ? w.row0 + 31 : last, G));
-    const int nt = (vmax + 31) >> 5, per = (nt + nsplit - 1) / nsplit;
+    const int nt = (vmax + 31) >> 5, per = split_tiles(p, nt, 32, nsplit);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
-    typename TL::Rows rw;
-    rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
     typename TL::template Fetch<NI> fk, fv;
     fk.init(lane, 0, 1, p.ldk, [](int r) { return TL::fk(r); });
     fv.init(lane, 0, 1, p.ldv, [](int r) { return TL::fv(r); });
@@ -496,6 +524,8 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
     };
     int st = 0, again = 0;
     if (t0 + wave < t1) issue(t0 + wave, 0);
+    typename TL::Rows rw;                                                          // (its loads and the first tile's are one trip to memory)
+    rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
     if (t0 + wave + NW < t1) issue(t0 + wave + NW, 1);
     for (int t = t0 + wave; t < t1; t += NW, st ^= 1) {
         if (t + NW < t1) { DEFT_WAVE_VM(2 * NI); } else { DEFT_WAVE_VM(0); }       // this wave's tile t is here (the stages are its own: no barrier)
@@ -516,7 +546,8 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
         }
     }
     if constexpr (NW == 1) {
-        write_rows<DT, D>(p, w, rw, nsplit, query, head, row <= last, h);
+        DEFT_WAVE_LGKM();
+        write_rows<DT, D>(p, w, rw, nsplit, query, head, w.rows - w.row0, lane, lds);
         return;
     }
     // join the waves: everybody's M and L, then O scaled to the common M, summed in wave order
@@ -580,8 +611,8 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(DeftAttn p, int nsplit)
     float L = x.y * al, o0 = 0.f, o1 = 0.f;
     for (int i = 1; i < 64; i <<= 1) L += __shfl_xor(L, i);
     const int col = lane * 2 < p.D ? lane * 2 : 0;
-#pragma unroll 4
-    for (int s = 0; s < nsplit; ++s) {
+    for (unsigned long long some = deft_ballot(x.y != 0.f); some; some &= some - 1) {             // (splits that saw keys of this row)
+        const int s = __builtin_ctzll(some);
         const float2 y = *(const float2*)(p.ws + ws_row(p, s, q, h) * p.D + col);
         const float a = __shfl(al, s);
         o0 = fmaf(y.x, a, o0);
@@ -629,7 +660,7 @@ Choice choose(const DeftAttn* d) {
     // rows that are there fill about this many workgroups
     const long long busy = ((long long)d->Tq * G / bm + (c.step ? d->B : d->B / 2 + 1)) * d->Hk;
     const int keys = c.step ? 256 : 512;                           // keys a split should have at least
-    long long want = busy < 512 ? (1024 + busy - 1) / busy : 1;
+    long long want = c.step ? 2048 / busy : 512 / busy;
     const long long most = ((long long)d->max_k + keys - 1) / keys;
     if (want > most) want = most;
     if (want > 64) want = 64;
