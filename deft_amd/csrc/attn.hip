@@ -69,48 +69,67 @@ struct Work {
     int b, hk, split;
     int q0, n, m;                 // first query, queries, keys
     int row0, rows;               // first row of the tile, rows of the sequence (n * G)
+    int qi, rem;                  // row0 = qi * G + rem
     const char *k, *v;            // key 0 / value 0 of this kv head
 };
+// The launch grid: x = kv head + Hk * split (neighbouring workgroups, on different XCDs, read different heads), y and z the flat tiles.
+struct Grid { int nsplit, ntiles; unsigned inv_g, inv_hk; };      // inv: 2^32 / n + 1, for quotients of small numbers (div_small)
+// x / n for x < 2^19, n <= 4096: inv n = 2^32 + e with 0 < e <= n, and x e < 2^32
+__device__ __forceinline__ int div_small(int x, unsigned inv) { return inv == 0 ? x : (int)__umulhi((unsigned)x, inv); }      // (inv = 0: n = 1)
 
 // Flat tile t -> (sequence, tile of it).  Sequence b starts at flat tile  first(b) = q_start[b] * G / BM + b,  which leaves it at least ceil(n G / BM)
 // tiles whatever the lengths are: no table of lengths is needed on the host, surplus tiles end at once.
 template <int BM>
-__device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, unsigned id, int nsplit, int ntiles, Work& w) {
+__device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, const Grid& g, Work& w) {
     const int G = p.Hq / p.Hk, lane = threadIdx.x & 63;
-    w.hk = (int)(id % (unsigned)p.Hk);                           // neighbouring workgroups (different XCDs) read different heads
-    id /= (unsigned)p.Hk;
-    w.split = nsplit == 1 ? 0 : (int)(id % (unsigned)nsplit);
-    const int t = ntiles - 1 - (int)(nsplit == 1 ? id : id / (unsigned)nsplit);      // causal: the long rows of a sequence first
-    // the last b with first(b) <= t (first() grows): down to 512 candidates 64 at a time, then 8 loads a lane at once -- one trip to memory, not three
-    auto before = [&](int at) { return clampi(p.q_start[at], 0, p.Tq) * G / BM + at <= t; };      // (Tq * Hq < 2^30)
+    w.split = g.nsplit == 1 ? 0 : div_small((int)blockIdx.x, g.inv_hk);
+    w.hk = (int)blockIdx.x - w.split * p.Hk;
+    const int t = g.ntiles - 1 - (int)(blockIdx.y + blockIdx.z * gridDim.y);         // causal: the long rows of a sequence first
+    if (t < 0) return false;
+    // the last b with first(b) <= t (first() grows): down to 448 candidates 64 at a time, then 8 loads a lane at once -- one trip to memory, which
+    // brings q_start[b] and q_start[b + 1] as well
+    auto start = [&](int at) { return clampi(p.q_start[at], 0, p.Tq); };
+    auto before = [&](int q, int at) { return q * G / BM + at <= t; };               // (Tq * Hq < 2^30)
     int lo = 0, n = p.B;
-    while (n > 512) {
+    while (n > 448) {
         const int step = (n + 63) >> 6, at = lo + lane * step;
-        const int c = __popcll(deft_ballot(at < lo + n && before(at)));
+        const int c = __popcll(deft_ballot(at < lo + n && before(start(at), at)));
         if (c == 0) return false;
         const int left = n - (c - 1) * step;
         lo += (c - 1) * step;
         n = left < step ? left : step;
     }
-    int c = 0;
-    if (n <= 64) c = __popcll(deft_ballot(lane < n && before(lo + (lane < n ? lane : 0))));
-    else {
-        bool le[8];
+    int c = 0, q0 = 0, q1 = 0;
+    if (n < 64) {
+        const int q = start(lo + (lane < n ? lane : n));
+        c = __popcll(deft_ballot(lane < n && before(q, lo + lane)));
+        if (c == 0) return false;
+        q0 = __shfl(q, c - 1);
+        q1 = __shfl(q, c);
+    } else {
+        int q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) le[i] = before(lo + (i * 64 + lane < n ? i * 64 + lane : 0));
+        for (int i = 0; i < 8; ++i) q[i] = start(lo + (i * 64 + lane < n ? i * 64 + lane : n));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c += __popcll(deft_ballot(i * 64 + lane < n && le[i]));
+        for (int i = 0; i < 8; ++i) c += __popcll(deft_ballot(i * 64 + lane < n && before(q[i], lo + i * 64 + lane)));
+        if (c == 0) return false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int a = __shfl(q[i], (c - 1) & 63), b = __shfl(q[i], c & 63);
+            q0 = (c - 1) >> 6 == i ? a : q0;
+            q1 = c >> 6 == i ? b : q1;
+        }
     }
-    if (c == 0) return false;
-    lo += c - 1;
-    const int b = w.b = __builtin_amdgcn_readfirstlane(lo);
-    w.q0 = clampi(p.q_start[b], 0, p.Tq);
-    w.n = clampi(p.q_start[b + 1], 0, p.Tq) - w.q0;
+    const int b = w.b = __builtin_amdgcn_readfirstlane(lo + c - 1);
+    w.q0 = __builtin_amdgcn_readfirstlane(q0);
+    w.n = __builtin_amdgcn_readfirstlane(q1) - w.q0;
     if (w.n <= 0) return false;
     w.rows = w.n * G;
     const int tile = t - (w.q0 * G / BM + b);
     if (tile >= (w.rows + BM - 1) / BM) return false;
     w.row0 = tile * BM;
+    w.qi = G == 1 ? w.row0 : w.row0 / G;
+    w.rem = w.row0 - w.qi * G;
     int m = p.k_len ? p.k_len[b] : w.n;
     const int at = p.k_start ? p.k_start[b] : w.q0;
     const bool there = at >= 0 && at < p.slots;
@@ -121,10 +140,8 @@ __device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, unsigned
     w.v = (const char*)p.v + (vo + (long long)w.hk * p.hsv) * tsize;
     return true;
 }
-// keys the row sees (j < vis)
-__device__ __forceinline__ int visible(const DeftAttn& p, const Work& w, int row, int G) {
-    return p.causal ? clampi(w.m - w.n + row / G + 1, 0, w.m) : w.m;
-}
+// keys (j < vis) that query i of the sequence sees
+__device__ __forceinline__ int visible(const DeftAttn& p, const Work& w, int i) { return p.causal ? clampi(w.m - w.n + i + 1, 0, w.m) : w.m; }
 
 // A tile of BN keys in LDS: rows of RB bytes, 16-byte chunks; chunk c of row r sits at slot c ^ f(r).
 //   K is read 16 bytes a lane, 32 rows at one chunk (served in groups of 16 lanes): f spreads the 16 rows of such a group over the 16 slots of the
@@ -426,25 +443,26 @@ __device__ __forceinline__ void write_rows(const DeftAttn& p, const Work& w, typ
 constexpr int BM = 128;
 
 template <int DT, int D>
-__global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, int nsplit, int ntiles) {
+__global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid grid) {
     typedef Tile<DT, D> TL;
     typedef typename TL::T T;
     constexpr int NT = DT == DEFT_F32 ? 1 : 2, BN = 32 * NT, KB = BN * TL::RB, NI = BN * TL::CPR / 256;
     static_assert(NI * 256 == BN * TL::CPR, "whole DMA instructions");
-    __shared__ __attribute__((aligned(1024))) char lds[4 * KB];                    // K, K, V, V
+    __shared__ __attribute__((aligned(1024))) char lds[4 * KB];                    // K and V of two stages (three were no faster: 124 -> 127 us, D = 64)
     __shared__ int again;
     const int G = p.Hq / p.Hk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     Work w;
-    if (!find_work<BM>(p, TL::TS, blockIdx.x, nsplit, ntiles, w)) return;
+    if (!find_work<BM>(p, TL::TS, grid, w)) return;
+    const int nsplit = grid.nsplit;
     const float sc = p.scale * LOG2E;
-    const int wr0 = w.row0 + wave * 32, row = wr0 + (lane & 31);
-    const int rc = row < w.rows ? row : w.rows - 1, query = w.q0 + rc / G, head = w.hk * G + rc % G;
-    const bool on = wr0 < w.rows;                                                  // this wave has rows
-    const int last = w.rows - 1;
-    const int vis = visible(p, w, rc, G);
-    const int vmin = __builtin_amdgcn_readfirstlane(visible(p, w, wr0 < last ? wr0 : last, G));               // the wave's first and last row
-    const int vmax = __builtin_amdgcn_readfirstlane(visible(p, w, wr0 + 31 < last ? wr0 + 31 : last, G));
-    const int bmax = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0 + BM - 1 < last ? w.row0 + BM - 1 : last, G));
+    const int left = w.rows - w.row0 - 1, wr0 = wave * 32;                         // the tile's last row, the wave's first
+    const bool on = wr0 <= left;                                                   // this wave has rows
+    auto query_of = [&](int r) { return w.qi + div_small(w.rem + (r < left ? r : left), grid.inv_g); };      // of row r of the tile (the last one's behind it)
+    const int rc = wr0 + (lane & 31) < left ? wr0 + (lane & 31) : left, qi = query_of(rc), query = w.q0 + qi;
+    const int head = w.hk * G + w.rem + rc - (qi - w.qi) * G;
+    const int vis = visible(p, w, qi);
+    const int vmin = visible(p, w, query_of(wr0)), vmax = visible(p, w, query_of(wr0 + 31));                  // the wave's first and last row
+    const int bmax = visible(p, w, query_of(BM - 1));
     const int nt = (bmax + BN - 1) / BN, per = split_tiles(p, nt, BN, nsplit);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
@@ -453,46 +471,44 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, int nsp
     fv.init(lane, wave, 4, p.ldv, [](int r) { return TL::fv(r); });
     const int kr = (int)p.ldk * TL::TS, vr = (int)p.ldv * TL::TS;                  // bytes between keys (<= 2^24)
     const lds_at base = lds_address(lds);
-    auto issue = [&](int t) {
+    auto issue = [&](int t, int st) {
         const int nv = w.m - t * BN;
-        fk.issue(w.k + (long long)t * BN * kr, base + (t & 1) * KB, wave, 4, nv, kr);
-        fv.issue(w.v + (long long)t * BN * vr, base + 2 * KB + (t & 1) * KB, wave, 4, nv, vr);
+        fk.issue(w.k + (long long)t * BN * kr, base + st * 2 * KB, wave, 4, nv, kr);
+        fv.issue(w.v + (long long)t * BN * vr, base + st * 2 * KB + KB, wave, 4, nv, vr);
     };
     if (tid == 0) again = 0;
-    if (t0 < t1) issue(t0);
+    if (t0 < t1) issue(t0, 0);
     typename TL::Rows rw;                                                          // (its loads and the first tile's are one trip to memory)
     rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
-    for (int t = t0; t < t1; ++t) {
+    int st = 0;
+    for (int t = t0; t < t1; ++t, st ^= 1) {
         DEFT_PIPE_BARRIER(0);                                                      // tile t is here, and nobody reads tile t - 1 any more
-        if (t + 1 < t1) issue(t + 1);
+        if (t + 1 < t1) issue(t + 1, st ^ 1);
         const int k0 = t * BN;
+        const char* const ks = lds + st * 2 * KB;
         if (on && k0 < vmax) {
             const int end = k0 + BN < w.m ? k0 + BN : w.m;
-            if (TL::template step<NT, false>(rw, lds + (t & 1) * KB, lds + 2 * KB + (t & 1) * KB, vis - k0, vmin < k0 + BN, vmin < end, sc, lane)) again = 1;
+            if (TL::template step<NT, false>(rw, ks, ks + KB, vis - k0, vmin < k0 + BN, vmin < end, sc, lane)) again = 1;
         }
     }
-    if (p.causal) {
-        __syncthreads();
-        if (again) {                                                               // (rare: infinities or NaN behind the diagonal of some row)
-            rw.clear();
-            for (int t = t0; t < t1; ++t) {
-                __syncthreads();
-                issue(t);
-                DEFT_PIPE_BARRIER(0);
-                if (on && t * BN < vmax) TL::template step<NT, true>(rw, lds + (t & 1) * KB, lds + 2 * KB + (t & 1) * KB, vis - t * BN, true, false, sc, lane);
-            }
+    __syncthreads();
+    if (p.causal && again) {                                                       // (rare: infinities or NaN behind the diagonal of some row)
+        rw.clear();
+        for (int t = t0; t < t1; ++t) {
+            issue(t, 0);
+            DEFT_PIPE_BARRIER(0);
+            if (on && t * BN < vmax) TL::template step<NT, true>(rw, lds, lds + KB, vis - t * BN, true, false, sc, lane);
             __syncthreads();
         }
     }
-    if (!p.causal) __syncthreads();                                                // (nobody reads the stages any more)
-    write_rows<DT, D>(p, w, rw, nsplit, query, head, w.rows - wr0, lane, lds + wave * KB);
+    write_rows<DT, D>(p, w, rw, nsplit, query, head, left + 1 - wr0, lane, lds + wave * KB);
 }
 
 // waves that share the keys of a row tile: two 32-key stages of K and V each stay within 128 KB
 template <int DT, int D> constexpr int step_waves() { return Tile<DT, D>::RB > 256 ? 2 : 4; }
 
 template <int DT, int D, int NW>
-__global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(DeftAttn p, int nsplit, int ntiles) {
+__global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(DeftAttn p, Grid grid) {
     typedef Tile<DT, D> TL;
     typedef typename TL::T T;
     constexpr int KB = 32 * TL::RB, LDS = NW * 4 * KB, NI = TL::CPR / 2;
@@ -501,13 +517,13 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
     __shared__ float ms[NW][32], ls[NW][32];
     const int G = p.Hq / p.Hk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
     Work w;
-    if (!find_work<32>(p, TL::TS, blockIdx.x, nsplit, ntiles, w)) return;
+    if (!find_work<32>(p, TL::TS, grid, w)) return;
+    const int nsplit = grid.nsplit;
     const float sc = p.scale * LOG2E;
-    const int last = w.rows - 1, row = w.row0 + l32, rc = row < last ? row : last;
-    const int query = w.q0 + rc / G, head = w.hk * G + rc % G;
-    const int vis = visible(p, w, rc, G);
-    const int vmin = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0, G));
-    const int vmax = __builtin_amdgcn_readfirstlane(visible(p, w, w.row0 + 31 < last ? w.row0 + 31 : last, G));
+    const int left = w.rows - w.row0 - 1;                                          // the tile's last row
+    auto query_of = [&](int r) { return w.qi + div_small(w.rem + (r < left ? r : left), grid.inv_g); };      // of row r of the tile (the last one's behind it)
+    const int rc = l32 < left ? l32 : left, qi = query_of(rc), query = w.q0 + qi, head = w.hk * G + w.rem + rc - (qi - w.qi) * G;
+    const int vis = visible(p, w, qi), vmin = visible(p, w, w.qi), vmax = visible(p, w, query_of(31));
     const int nt = (vmax + 31) >> 5, per = split_tiles(p, nt, 32, nsplit);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
@@ -547,7 +563,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
     }
     if constexpr (NW == 1) {
         DEFT_WAVE_LGKM();
-        write_rows<DT, D>(p, w, rw, nsplit, query, head, w.rows - w.row0, lane, lds);
+        write_rows<DT, D>(p, w, rw, nsplit, query, head, left + 1, lane, lds);
         return;
     }
     // join the waves: everybody's M and L, then O scaled to the common M, summed in wave order
@@ -565,7 +581,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
         for (int r = 0; r < 16; ++r) os[(wave * D + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3)) * 32 + l32] = rw.o[j][r] * al;
     __syncthreads();
     // thread: a row's chunk of 4 columns
-    const int nrows = w.rows - w.row0 < 32 ? w.rows - w.row0 : 32;
+    const int nrows = left < 31 ? left + 1 : 32;
     for (int it = tid; it < nrows * (D / 4); it += 64 * NW) {
         const int r = it / (D / 4), c = (it - r * (D / 4)) * 4;
         float Mr = ms[0][r];
@@ -579,7 +595,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] += os[(i * D + c + e) * 32 + r];
         }
-        const int qr = w.q0 + (w.row0 + r) / G, hd = w.hk * G + (w.row0 + r) % G;
+        const int iq = query_of(r), qr = w.q0 + iq, hd = w.hk * G + w.rem + r - (iq - w.qi) * G;
         if (nsplit > 1) {
             *(f32x4*)(p.ws + ws_row(p, w.split, qr, hd) * D + c) = x;
             if (c == 0) *(float2*)(ws_ml(p, nsplit) + ws_row(p, w.split, qr, hd) * 2) = make_float2(Mr, Lr);
@@ -653,7 +669,7 @@ struct Choice { bool step; int waves, nsplit, ntiles; };
 Choice choose(const DeftAttn* d) {
     const int G = d->Hq / d->Hk;
     Choice c;
-    c.step = (long long)d->Tq * G <= 32ll * d->B;                  // up to 32 rows a sequence on average
+    c.step = (long long)d->Tq * G <= 32ll * d->B || d->max_k <= 64;
     const int bm = c.step ? 32 : BM;
     c.ntiles = d->Tq * G / bm + d->B;                              // (below 2^26 + 2^24)
     c.waves = !c.step ? 4 : d->max_k <= 64 ? 1 : d->dtype == DEFT_F32 && d->D > 64 ? 2 : 4;
@@ -668,26 +684,28 @@ Choice choose(const DeftAttn* d) {
     return c;
 }
 
+struct Launch { Choice c; Grid g; dim3 grid; hipStream_t s; };
 template <int DT, int D>
-void attn_launch(const DeftAttn& d, const Choice& c, unsigned grid, hipStream_t s) {
+void attn_launch(const DeftAttn& d, const Launch& l) {
     constexpr int NW = step_waves<DT, D>();
-    if (!c.step) hipLaunchKernelGGL((attn_prompt_kernel<DT, D>), dim3(grid), dim3(256), 0, s, d, c.nsplit, c.ntiles);
-    else if (c.waves == 1) hipLaunchKernelGGL((attn_step_kernel<DT, D, 1>), dim3(grid), dim3(64), 0, s, d, c.nsplit, c.ntiles);
-    else hipLaunchKernelGGL((attn_step_kernel<DT, D, NW>), dim3(grid), dim3(64 * NW), 0, s, d, c.nsplit, c.ntiles);
+    if (!l.c.step) hipLaunchKernelGGL((attn_prompt_kernel<DT, D>), l.grid, dim3(256), 0, l.s, d, l.g);
+    else if (l.c.waves == 1) hipLaunchKernelGGL((attn_step_kernel<DT, D, 1>), l.grid, dim3(64), 0, l.s, d, l.g);
+    else hipLaunchKernelGGL((attn_step_kernel<DT, D, NW>), l.grid, dim3(64 * NW), 0, l.s, d, l.g);
 }
 template <int DT>
-void attn_launch_d(const DeftAttn& d, const Choice& c, unsigned grid, hipStream_t s) {
+void attn_launch_d(const DeftAttn& d, const Launch& l) {
     switch (d.D) {
-        case 32: attn_launch<DT, 32>(d, c, grid, s); break;
-        case 64: attn_launch<DT, 64>(d, c, grid, s); break;
-        case 96: attn_launch<DT, 96>(d, c, grid, s); break;
-        default: attn_launch<DT, 128>(d, c, grid, s);
+        case 32: attn_launch<DT, 32>(d, l); break;
+        case 64: attn_launch<DT, 64>(d, l); break;
+        case 96: attn_launch<DT, 96>(d, l); break;
+        default: attn_launch<DT, 128>(d, l);
     }
-    if (c.nsplit > 1) {
+    if (l.g.nsplit > 1) {
         const unsigned mg = (unsigned)(((long long)d.Tq * d.Hq + 3) / 4);
-        hipLaunchKernelGGL((attn_merge_kernel<DT>), dim3(mg), dim3(256), 0, s, d, c.nsplit);
+        hipLaunchKernelGGL((attn_merge_kernel<DT>), dim3(mg), dim3(256), 0, l.s, d, l.g.nsplit);
     }
 }
+unsigned inverse(int n) { return n == 1 ? 0u : (unsigned)(0x100000000ull / (unsigned)n + 1); }
 
 }  // namespace
 
@@ -707,12 +725,15 @@ extern "C" int deft_attn(const DeftAttn* d, void* stream) {
     const long long need = c.nsplit > 1 ? (long long)c.nsplit * d->Tq * d->Hq * (d->D + 2) : 0;
     DEFT_CHECK(need == 0 || (d->ws && d->ws_floats >= need && ((size_t)d->ws & 15) == 0), -139, "deft_attn: workspace of %lld floats, 16-byte aligned, has %lld", need,
                d->ws ? d->ws_floats : 0ll);
-    const long long grid = (long long)c.ntiles * c.nsplit * d->Hk;
-    DEFT_CHECK(grid < (1ll << 31), -134, "deft_attn: %lld workgroups", grid);
-    hipStream_t s = (hipStream_t)stream;
-    if (d->dtype == DEFT_F32) attn_launch_d<DEFT_F32>(*d, c, (unsigned)grid, s);
-    else if (d->dtype == DEFT_F16) attn_launch_d<DEFT_F16>(*d, c, (unsigned)grid, s);
-    else attn_launch_d<DEFT_BF16>(*d, c, (unsigned)grid, s);
+    Launch l;
+    l.c = c;
+    l.g = Grid{c.nsplit, c.ntiles, inverse(d->Hq / d->Hk), inverse(d->Hk)};
+    const int y = c.ntiles < 32768 ? c.ntiles : 32768;
+    l.grid = dim3((unsigned)(d->Hk * c.nsplit), (unsigned)y, (unsigned)((c.ntiles + y - 1) / y));
+    l.s = (hipStream_t)stream;
+    if (d->dtype == DEFT_F32) attn_launch_d<DEFT_F32>(*d, l);
+    else if (d->dtype == DEFT_F16) attn_launch_d<DEFT_F16>(*d, l);
+    else attn_launch_d<DEFT_BF16>(*d, l);
     DEFT_CHECK_LAUNCH("attn");
     return 0;
 }

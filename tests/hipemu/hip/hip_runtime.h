@@ -538,6 +538,7 @@ template <int S> static inline float deft_add_xor(float v) { return v + __shfl_x
 static inline float deft_rsq(float x) { return 1.f / sqrtf(x); }
 static inline float deft_exp2(float x) { return exp2f(x); }
 static inline float deft_log2(float x) { return log2f(x); }
+static inline unsigned __umulhi(unsigned a, unsigned b) { return (unsigned)(((unsigned long long)a * b) >> 32); }
 static inline int __popcll(unsigned long long x) { return __builtin_popcountll(x); }
 extern "C" __attribute__((weak, visibility("default"))) void hipemu_set_late_dma(int on) { hipemu::late_dma() = on; }
 #define DEFT_OPAQUE(v) ((void)(v))
