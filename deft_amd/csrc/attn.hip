@@ -504,16 +504,18 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
     write_rows<DT, D>(p, w, rw, nsplit, query, head, left + 1 - wr0, lane, lds + wave * KB);
 }
 
-// waves that share the keys of a row tile: two 32-key stages of K and V each stay within 128 KB
+// waves that share the keys of a row tile (or one): two 32-key stages of K and V each stay within 128 KB
 template <int DT, int D> constexpr int step_waves() { return Tile<DT, D>::RB > 256 ? 2 : 4; }
 
 template <int DT, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(DeftAttn p, Grid grid) {
     typedef Tile<DT, D> TL;
     typedef typename TL::T T;
-    constexpr int KB = 32 * TL::RB, LDS = NW * 4 * KB, NI = TL::CPR / 2;
-    static_assert(LDS >= NW * 32 * D * 4, "the join fits the stages");
-    __shared__ __attribute__((aligned(1024))) char lds[LDS];
+    // one wave: one or two key tiles, one stage -- twice the workgroups on a compute unit are worth more than the overlap (500 fp32 histories of up
+    // to 50: 20.5 us against 23.5 with two); else two
+    constexpr int NS = NW == 1 ? 1 : 2, KB = 32 * TL::RB, WB = NS * 2 * KB, NI = TL::CPR / 2;
+    static_assert(WB >= 32 * D * 4, "a wave's rows fit its stages");
+    __shared__ __attribute__((aligned(1024))) char lds[NW * WB];                // per wave: K, V of stage 0, K, V of stage 1
     __shared__ float ms[NW][32], ls[NW][32];
     const int G = p.Hq / p.Hk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l32 = lane & 31;
     Work w;
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
     typename TL::template Fetch<NI> fk, fv;
     fk.init(lane, 0, 1, p.ldk, [](int r) { return TL::fk(r); });
     fv.init(lane, 0, 1, p.ldv, [](int r) { return TL::fv(r); });
-    char* const mine = lds + wave * 4 * KB;                                        // K, V of stage 0, K, V of stage 1
+    char* const mine = lds + wave * WB;
     const int kr = (int)p.ldk * TL::TS, vr = (int)p.ldv * TL::TS;                  // bytes between keys (<= 2^24)
     const lds_at base = lds_address(mine);
     auto issue = [&](int t, int st) {
@@ -542,14 +544,14 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
     if (t0 + wave < t1) issue(t0 + wave, 0);
     typename TL::Rows rw;                                                          // (its loads and the first tile's are one trip to memory)
     rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
-    if (t0 + wave + NW < t1) issue(t0 + wave + NW, 1);
-    for (int t = t0 + wave; t < t1; t += NW, st ^= 1) {
-        if (t + NW < t1) { DEFT_WAVE_VM(2 * NI); } else { DEFT_WAVE_VM(0); }       // this wave's tile t is here (the stages are its own: no barrier)
+    if (NS == 2 && t0 + wave + NW < t1) issue(t0 + wave + NW, 1);
+    for (int t = t0 + wave; t < t1; t += NW, st ^= NS - 1) {
+        if (NS == 2 && t + NW < t1) { DEFT_WAVE_VM(2 * NI); } else { DEFT_WAVE_VM(0); }       // this wave's tile t is here (the stages are its own: no barrier)
         const int k0 = t * 32, end = k0 + 32 < w.m ? k0 + 32 : w.m;
         if (TL::template step<1, false>(rw, mine + st * 2 * KB, mine + st * 2 * KB + KB, vis - k0, vmin < k0 + 32, vmin < end, sc, lane)) again = 1;
-        if (t + 2 * NW < t1) {
+        if (t + NS * NW < t1) {
             DEFT_WAVE_LGKM();                                                      // its reads have returned: the stage may be filled again
-            issue(t + 2 * NW, st);
+            issue(t + NS * NW, st);
         }
     }
     if (again) {                                                                   // (rare: infinities or NaN behind the diagonal of some row)
