@@ -204,8 +204,8 @@ class AttentionPlan(_Plan):
         k, v [slots][cap][kv_heads][D]: a cache; its keys are the k_len[b] first rows of slot slot[b].
         causal: query i of n sees the keys j <= m - n + i of its m (a lone new token sees all of them).  Rows that see no key give 0; rows of no
         sequence are not written.  Starts, lengths and slots are int32 device tensors, clamped to the tensors by the kernel; max_k (host): an
-        estimate of the longest m, which steers only how the work is split (default: a cache's cap, the number of packed key rows, or twice the
-        average length where keys are the queries' own rows).
+        estimate of the longest m, which steers only how the work is split (default: a cache's cap, the number of packed key rows, or the average
+        length where keys are the queries' own rows).
         lse=True: returns (o, lse [Tq][heads] float32), the log of each row's sum of exponentials (-inf where it sees no key)."""
         H, Hk, D, dt = self.heads, self.kv_heads, self.head_dim, getattr(q, "dtype", None)
         if dt not in _DTYPE:
@@ -230,7 +230,7 @@ class AttentionPlan(_Plan):
             if k_start is not None:
                 sp = self._ints("k_start", k_start, B)
             elif k_len is None and B > 1:
-                longest = min(longest, 2 * Tq // B + 1)
+                longest = min(longest, Tq // B + 1)
         if k.shape != v.shape:
             _refuse(True, "k has shape %s, v %s", tuple(k.shape), tuple(v.shape))
         lp = self._ints("k_len", k_len, B) if k_len is not None else 0

@@ -504,16 +504,13 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
     write_rows<DT, D>(p, w, rw, nsplit, query, head, left + 1 - wr0, lane, lds + wave * KB);
 }
 
-// waves that share the keys of a row tile (or one): two 32-key stages of K and V each stay within 128 KB
-template <int DT, int D> constexpr int step_waves() { return Tile<DT, D>::RB > 256 ? 2 : 4; }
-
 template <int DT, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(DeftAttn p, Grid grid) {
     typedef Tile<DT, D> TL;
     typedef typename TL::T T;
-    // one wave: one or two key tiles, one stage -- twice the workgroups on a compute unit are worth more than the overlap (500 fp32 histories of up
-    // to 50: 20.5 us against 23.5 with two); else two
-    constexpr int NS = NW == 1 ? 1 : 2, KB = 32 * TL::RB, WB = NS * 2 * KB, NI = TL::CPR / 2;
+    // One wave: one stage -- twice the workgroups on a compute unit are worth more than the overlap (500 fp32 histories of up to 50: 20.5 us against
+    // 23.5 with two).  Four: two stages where they fit 128 KB; fp32 of D = 96, 128 takes one for the fourth wave (its matrix products are the cost).
+    constexpr int NS = NW == 1 || TL::RB > 256 ? 1 : 2, KB = 32 * TL::RB, WB = NS * 2 * KB, NI = TL::CPR / 2;
     static_assert(WB >= 32 * D * 4, "a wave's rows fit its stages");
     __shared__ __attribute__((aligned(1024))) char lds[NW * WB];                // per wave: K, V of stage 0, K, V of stage 1
     __shared__ float ms[NW][32], ls[NW][32];
@@ -674,11 +671,13 @@ Choice choose(const DeftAttn* d) {
     c.step = (long long)d->Tq * G <= 32ll * d->B || d->max_k <= 64;
     const int bm = c.step ? 32 : BM;
     c.ntiles = d->Tq * G / bm + d->B;                              // (below 2^26 + 2^24)
-    c.waves = !c.step ? 4 : d->max_k <= 64 ? 1 : d->dtype == DEFT_F32 && d->D > 64 ? 2 : 4;
-    // rows that are there fill about this many workgroups
+    // rows that are there fill about this many workgroups (tiles x heads)
     const long long busy = ((long long)d->Tq * G / bm + (c.step ? d->B : d->B / 2 + 1)) * d->Hk;
     const int keys = c.step ? 256 : 512;                           // keys a split should have at least
-    long long want = c.step ? 2048 / busy : 512 / busy;
+    // one wave a row tile where the keys are one or two tiles, or where that already fills the chip (256 x 8 heads over 100 .. 500 keys, D = 128: 71 us
+    // against 92 with four; 200 x 4 over 30 .. 120: 10.1 against 12.3; 256 x 4 over 500, D = 64: 22 against 21)
+    c.waves = c.step && (d->max_k <= 64 || (busy >= 800 && d->max_k <= 512)) ? 1 : 4;
+    long long want = c.step ? 2048 / busy : 768 / busy;
     const long long most = ((long long)d->max_k + keys - 1) / keys;
     if (want > most) want = most;
     if (want > 64) want = 64;
@@ -689,10 +688,9 @@ Choice choose(const DeftAttn* d) {
 struct Launch { Choice c; Grid g; dim3 grid; hipStream_t s; };
 template <int DT, int D>
 void attn_launch(const DeftAttn& d, const Launch& l) {
-    constexpr int NW = step_waves<DT, D>();
     if (!l.c.step) hipLaunchKernelGGL((attn_prompt_kernel<DT, D>), l.grid, dim3(256), 0, l.s, d, l.g);
     else if (l.c.waves == 1) hipLaunchKernelGGL((attn_step_kernel<DT, D, 1>), l.grid, dim3(64), 0, l.s, d, l.g);
-    else hipLaunchKernelGGL((attn_step_kernel<DT, D, NW>), l.grid, dim3(64 * NW), 0, l.s, d, l.g);
+    else hipLaunchKernelGGL((attn_step_kernel<DT, D, 4>), l.grid, dim3(256), 0, l.s, d, l.g);
 }
 template <int DT>
 void attn_launch_d(const DeftAttn& d, const Launch& l) {
