@@ -79,22 +79,23 @@ class AttentionPlan(_Plan):
         try:
             T, h, D = x.shape
             ld, hs, one = x.stride()
-            if h == heads and D == self.head_dim and x.dtype is dtype and one == 1 and (tokens is None or T == tokens) and x.get_device() == self._index:
+            if h == heads and D == self.head_dim and x.dtype is dtype and one == 1 and (tokens is None or T == tokens) and x.get_device() == self._index \
+                    and not x.requires_grad:
                 return 0 if T == 1 else ld, 0 if h == 1 else hs          # (the stride of a one-long dimension says nothing)
         except (AttributeError, ValueError, TypeError):
             pass
-        self._not_rows(name, x, heads, dtype, tokens, "[tokens]")
+        return self._not_rows(name, x, heads, dtype, tokens, "[tokens]")
 
     def _slots(self, name, x, dtype):
         """(slot stride, row stride, head stride) of a cache x [slots][rows][kv_heads][head_dim]."""
         try:
             S, cap, h, D = x.shape
             ss, ld, hs, one = x.stride()
-            if h == self.kv_heads and D == self.head_dim and x.dtype is dtype and one == 1 and x.get_device() == self._index:
+            if h == self.kv_heads and D == self.head_dim and x.dtype is dtype and one == 1 and x.get_device() == self._index and not x.requires_grad:
                 return 0 if S == 1 else ss, 0 if cap == 1 else ld, 0 if h == 1 else hs
         except (AttributeError, ValueError, TypeError):
             pass
-        self._not_rows(name, x, self.kv_heads, dtype, None, "[slots][rows]")
+        return self._not_rows(name, x, self.kv_heads, dtype, None, "[slots][rows]")
 
     def _not_rows(self, name, x, heads, dtype, tokens, lead):
         _refuse(not isinstance(x, torch.Tensor), "%s is not a tensor", name)
@@ -103,7 +104,9 @@ class AttentionPlan(_Plan):
         _refuse(x.dtype is not dtype, "%s is %s, wanted %s", name, x.dtype, dtype)
         _refuse(x.get_device() != self._index, "%s is on %s, the plan on %s", name, x.device, self.device)
         _refuse(tokens is not None and x.shape[0] != tokens, "%s has %d tokens, wanted %s", name, x.shape[0], tokens)
-        _refuse(True, "%s: elements of a head must be contiguous", name)
+        _refuse(x.stride(-1) != 1, "%s: elements of a head must be contiguous", name)
+        _refuse(torch.is_grad_enabled(), "%s requires a gradient: these operators are forward only (torch.no_grad, or detach)", name)
+        return self._rows(name, x.detach(), heads, dtype, tokens) if lead == "[tokens]" else self._slots(name, x.detach(), dtype)
 
     def _ints(self, name, x, n):
         """Address of n int32 values on the plan's device."""
@@ -124,9 +127,9 @@ class AttentionPlan(_Plan):
     # ---- rotary positions, norms ---------------------------------------------------------------------------------------------------------
     def rotate(self, q, k, pos, v=None, cache=None, row=None, out=None, inverse=False):
         """Turns q [T][heads][D] and k [T][kv_heads][D] (None: queries only) by their positions pos [T][axes] (int32, or float32 for sub-pixel
-        centres).  Returns (q', k'): new tensors, or `out` = (q_out, k_out) (which may be q and k themselves).  cache = (k_cache, v_cache) with
+        centres).  Returns (q', k'): new tensors, or `out` = (q_out, k_out) (which may be q and k themselves, and must not overlap them otherwise).  cache = (k_cache, v_cache) with
         row [T] int32: token t's key -- and value, with v [T][kv_heads][D] -- are written to row row[t] of the caches ([rows] or [slots][rows]
-        [kv_heads][D]; a row outside is skipped, no two tokens may share one) and k' is the key cache.  inverse: turns back."""
+        [kv_heads][D]; a row outside is skipped, no two tokens may share one, the caches overlap no input) and k' is the key cache.  inverse: turns back."""
         return self._rotary(q, k, pos, v, cache, row, out, inverse, False)
 
     def norm_rotate(self, q, k, pos, v=None, cache=None, row=None, out=None):

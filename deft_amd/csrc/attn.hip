@@ -38,8 +38,10 @@ __device__ __forceinline__ lds_at lds_address(char* lds) { return (unsigned)(siz
 // `bytes` from `base` on may be read, chunks behind them arrive as zeros
 __device__ __forceinline__ lds_src lds_source(const char* base, unsigned bytes) {
     const unsigned long long a = (unsigned long long)base;
-    return lds_src{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)),
-                   (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+    lds_src s = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)),
+                 (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+    asm volatile("s_nop 4" : "+s"(s));               // (five wait states from a vector write of a scalar register to a memory instruction that reads it)
+    return s;
 }
 __device__ __forceinline__ void lds_fetch(const lds_src& s, lds_at lds, unsigned off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(s) : "memory", "m0");
@@ -73,7 +75,7 @@ struct Work {
     const char *k, *v;            // key 0 / value 0 of this kv head
 };
 // The launch grid: x = kv head + Hk * split (neighbouring workgroups, on different XCDs, read different heads), y and z the flat tiles.
-struct Grid { int nsplit, ntiles; unsigned inv_g, inv_hk; };      // inv: 2^32 / n + 1, for quotients of small numbers (div_small)
+struct Grid { int nsplit, ntiles, piece; unsigned inv_g, inv_hk; };      // piece: see split_tiles; inv: 2^32 / n + 1, for quotients of small numbers (div_small)
 // x / n for x < 2^19, n <= 4096: inv n = 2^32 + e with 0 < e <= n, and x e < 2^32
 __device__ __forceinline__ int div_small(int x, unsigned inv) { return inv == 0 ? x : (int)__umulhi((unsigned)x, inv); }      // (inv = 0: n = 1)
 
@@ -377,11 +379,11 @@ struct Tile {
     }
 };
 
-// Key tiles (of bn keys) a split takes: a fixed piece, 1 / nsplit of the longest sequence, so that the workgroups of long and short sequences take
-// equally long (a short one's later splits have nothing to do); more where max_k was too low an estimate.
-__device__ __forceinline__ int split_tiles(const DeftAttn& p, int nt, int bn, int nsplit) {
-    const int even = (nt + nsplit - 1) / nsplit, fixed = nsplit == 1 ? even : ((p.max_k + bn - 1) / bn + nsplit - 1) / nsplit;
-    return even > fixed ? even : fixed;
+// Key tiles a split takes: a fixed piece, 1 / nsplit of the longest sequence, so that the workgroups of long and short sequences take equally
+// long (a short one's later splits have nothing to do); more where max_k was too low an estimate.
+__device__ __forceinline__ int split_tiles(const Grid& g, int nt) {
+    const int even = (nt + g.nsplit - 1) / g.nsplit;
+    return even > g.piece ? even : g.piece;
 }
 
 // Where a split's partial results stand in the workspace: O [split][row][D], then (M, L) [split][row]; row = query * Hq + head
@@ -463,7 +465,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
     const int vis = visible(p, w, qi);
     const int vmin = visible(p, w, query_of(wr0)), vmax = visible(p, w, query_of(wr0 + 31));                  // the wave's first and last row
     const int bmax = visible(p, w, query_of(BM - 1));
-    const int nt = (bmax + BN - 1) / BN, per = split_tiles(p, nt, BN, nsplit);
+    const int nt = (bmax + BN - 1) / BN, per = split_tiles(grid, nt);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
     typename TL::template Fetch<NI> fk, fv;
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(Def
     auto query_of = [&](int r) { return w.qi + div_small(w.rem + (r < left ? r : left), grid.inv_g); };      // of row r of the tile (the last one's behind it)
     const int rc = l32 < left ? l32 : left, qi = query_of(rc), query = w.q0 + qi, head = w.hk * G + w.rem + rc - (qi - w.qi) * G;
     const int vis = visible(p, w, qi), vmin = visible(p, w, w.qi), vmax = visible(p, w, query_of(31));
-    const int nt = (vmax + 31) >> 5, per = split_tiles(p, nt, 32, nsplit);
+    const int nt = (vmax + 31) >> 5, per = split_tiles(grid, nt);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
     typename TL::template Fetch<NI> fk, fv;
@@ -673,11 +675,12 @@ Choice choose(const DeftAttn* d) {
     c.ntiles = d->Tq * G / bm + d->B;                              // (below 2^26 + 2^24)
     // rows that are there fill about this many workgroups (tiles x heads)
     const long long busy = ((long long)d->Tq * G / bm + (c.step ? d->B : d->B / 2 + 1)) * d->Hk;
-    const int keys = c.step ? 256 : 512;                           // keys a split should have at least
+    const bool f32 = d->dtype == DEFT_F32;                         // (its products take 8 times as long: shorter pieces)
+    const int keys = c.step || f32 ? 256 : 512;                    // keys a split should have at least
     // one wave a row tile where the keys are one or two tiles, or where that already fills the chip (256 x 8 heads over 100 .. 500 keys, D = 128: 71 us
     // against 92 with four; 200 x 4 over 30 .. 120: 10.1 against 12.3; 256 x 4 over 500, D = 64: 22 against 21)
     c.waves = c.step && (d->max_k <= 64 || (busy >= 800 && d->max_k <= 512)) ? 1 : 4;
-    long long want = c.step ? 2048 / busy : 768 / busy;
+    long long want = (c.step ? 2048 : 768) / busy;
     const long long most = ((long long)d->max_k + keys - 1) / keys;
     if (want > most) want = most;
     if (want > 64) want = 64;
@@ -727,7 +730,8 @@ extern "C" int deft_attn(const DeftAttn* d, void* stream) {
                d->ws ? d->ws_floats : 0ll);
     Launch l;
     l.c = c;
-    l.g = Grid{c.nsplit, c.ntiles, inverse(d->Hq / d->Hk), inverse(d->Hk)};
+    const int bn = c.step || d->dtype == DEFT_F32 ? 32 : 64;       // keys of a tile
+    l.g = Grid{c.nsplit, c.ntiles, c.nsplit == 1 ? 0 : deft_cdiv(((long long)d->max_k + bn - 1) / bn, c.nsplit), inverse(d->Hq / d->Hk), inverse(d->Hk)};
     const int y = c.ntiles < 32768 ? c.ntiles : 32768;
     l.grid = dim3((unsigned)(d->Hk * c.nsplit), (unsigned)y, (unsigned)((c.ntiles + y - 1) / y));
     l.s = (hipStream_t)stream;

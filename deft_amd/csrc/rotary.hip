@@ -229,6 +229,7 @@ extern "C" int deft_rotary(const DeftRotary* d, void* stream) {
     }
     DEFT_CHECK((al & 15) == 0, -124, "deft_rotary: pointers must be 16-byte aligned");
     DEFT_CHECK(fit, -125, "deft_rotary: strides must be multiples of %d elements and keep heads apart", V);
+    DEFT_CHECK(!d->norm || d->eps >= 0.f, -127, "deft_rotary: eps=%g", (double)d->eps);
     DEFT_CHECK(!d->row || d->rows >= 0, -126, "deft_rotary: rows=%lld", d->rows);
     if (d->T == 0) return 0;
     int lanes = 1;

@@ -404,7 +404,8 @@ long long deft_direct_weight_bytes(int KH, int KW, int Cin, int Cout);
  *   Pair i is elements (i, i + R), or (2i, 2i + 1) when `adjacent`; elements 2R .. D-1 are not turned.
  * pos [T][A]: int, or float when pos_float (sub-pixel centres).  q [T][Hq][D] -> q_out, k [T][Hk][D] -> k_out, v [T][Hk][D] -> v_out (copied
  * only); k and v may be NULL, v needs k.  row != NULL: token t's k / v go to row row[t] of k_out / v_out (a cache with `rows` rows); a row
- * outside 0 .. rows-1 is not written; two tokens of one call must not name the same row.  q_out = q and (without row) k_out = k are allowed.
+ * outside 0 .. rows-1 is not written; two tokens of one call must not name the same row.  q_out = q and (without row) k_out = k are allowed, other
+ * overlaps of inputs and outputs are not.
  * One rounding to the element type at the end.  D % 16 == 0 and R % 8 == 0 (fp32: 8 and 4), D <= 256. */
 typedef struct DeftRotary {
     const void *q, *k, *v;
@@ -428,7 +429,7 @@ int deft_rotary(const DeftRotary* d, void* stream);
  *   cache  (cap > 0):  rows 0 .. m-1 of slot k_start[b] of k / v [slots][cap][Hk][D] (slot strides ssk / ssv), m = k_len[b] -- the single-token
  *                      form: n = 1 query per track over its history
  * and query i sees key j when  !causal || j <= m - n + i.  o = softmax(scale * q k^T) v in fp32, rounded once; lse (NULL, or [Tq][Hq]
- * float) = log of the softmax's sum.  A row that sees no key gets o = 0 and lse = -inf.  Query rows of no sequence are left as they were.  Lengths
+ * float) = log of the softmax's sum.  A row that sees no key, or only scores of -inf, gets o = 0 and lse = -inf.  o must not overlap k or v.  Query rows of no sequence are left as they were.  Lengths
  * and starts are DEVICE data: they are clamped to the tensors (q_start to 0 .. Tq, keys to the rows of the slot / of k), never read past them,
  * and key rows >= m are never used, whatever they hold; a masked key takes no part even where its value is an infinity or NaN.
  * max_k is a host-side estimate of the longest m that steers only how the work is split; ws / ws_floats: workspace, at least

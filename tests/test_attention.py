@@ -151,6 +151,32 @@ def test_refusals(emu_lib):
             plan.attend(*args, **kw)
 
 
+def test_estimates_steer_only_the_split(dma):
+    """max_k wrong in either direction, every kernel: one wave or four, prompt or step, keys split or not."""
+    for dt in (F32, BF16):
+        for max_k in (1, 700, 2 ** 40):
+            ac.check_attend(dma, "cpu", dt, [1, 3], [330, 40], 2, 1, 64, cache="slots", poison=True, max_k=max_k)
+            ac.check_attend(dma, "cpu", dt, [80], [600], 1, 1, 32, max_k=max_k)
+            ac.check_attend(dma, "cpu", dt, [2, 40], [300, 40], 2, 2, 32, causal=False, cache="slots", max_k=max_k)
+
+
+def test_gradients_are_refused(emu_lib):
+    plan = AttentionPlan(2, 1, 32, axes=(16,), device="cpu", lib=emu_lib)
+    q, k, pos, qs = torch.ones(2, 2, 32, requires_grad=True), torch.ones(2, 1, 32), torch.zeros(2, 1, dtype=torch.int32), torch.tensor([0, 2], dtype=torch.int32)
+    for call in (lambda: plan.rotate(q, k, pos), lambda: plan.attend(q, k, k, qs), lambda: plan.attend(q.detach(), k, k.clone().requires_grad_(), qs)):
+        with pytest.raises(DeftHipError, match="forward only"):
+            call()
+    with torch.no_grad():
+        assert plan.attend(q, k, k, qs).shape == (2, 2, 32) and plan.rotate(q, k, pos)[0].shape == (2, 2, 32)
+
+
+def test_many_heads_and_sequences(emu_lib):
+    """More sequences than one lookup step takes, groups wider than a tile, gaps between nothing and nothing."""
+    ac.check_attend(emu_lib, "cpu", F32, [1, 0, 2] * 170, [3, 1, 2] * 170, 1, 1, 32)
+    ac.check_attend(emu_lib, "cpu", BF16, [3], [20], 150, 1, 32)
+    ac.check_attend(emu_lib, "cpu", BF16, [2, 3], [90, 3], 135, 3, 32, cache="slots")
+
+
 def test_descriptor_layouts_match_the_header():
     """ctypes mirrors of DeftRotary / DeftAttn: the header's fields in the header's order."""
     import os

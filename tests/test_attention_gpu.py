@@ -43,6 +43,43 @@ def test_attend(gpu_lib, dt, kw):
     ac.check_attend(gpu_lib, "cuda", dt, **kw)
 
 
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+def test_every_kernel(gpu_lib, dt, D):
+    """Prompt and step kernels of every width and type, one wave or four, keys split or whole, causal or not, lengths that end inside tiles."""
+    ac.check_attend(gpu_lib, "cuda", dt, [260, 33], [260, 33], 4, 2, D)                               # prompt
+    ac.check_attend(gpu_lib, "cuda", dt, [130], [1500], 2, 1, D)                                      # prompt, keys split
+    ac.check_attend(gpu_lib, "cuda", dt, [150, 90], [333, 90], 2, 1, D, causal=False, cache="slots", poison=True)
+    ac.check_attend(gpu_lib, "cuda", dt, [1, 1, 5], [60, 31, 5], 6, 2, D, cache="slots", poison=True)  # step, one wave
+    ac.check_attend(gpu_lib, "cuda", dt, [1, 2], [900, 255], 5, 1, D, cache="slots", poison=True)     # step, four waves, keys split
+    ac.check_attend(gpu_lib, "cuda", dt, [1, 2], [900, 255], 5, 1, D, cache="slots", poison=True, max_k=1)    # one wave over long keys
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_masked_keys_take_no_part(gpu_lib, dt, bad):
+    """Infinities and NaN in keys and values behind a row's last visible key: prompt and step kernel, whole and split."""
+    def spoil(b):
+        n = 0
+        for (k, v), q in zip(b["keys"], b["queries"]):
+            m = k.shape[0]
+            if "slot" not in b and m == q.shape[0]:
+                k[-1], v[-1], v[-2, :, ::3] = bad, bad, bad
+                b["k"][n:n + m], b["v"][n:n + m] = k.to("cuda"), v.to("cuda")
+            n += m
+    for nq in ([37, 5], [300, 4]):
+        b = ac.make_batch(dt, nq, nq, 2, 1, 64, "cuda", seed=2)
+        plan = AttentionPlan(2, 1, 64, device="cuda")
+        spoil(b)
+        for max_k in (None, 1000):
+            o = plan.attend(b["q"], b["k"], b["v"], b["q_start"], max_k=max_k)
+            for i, n in enumerate(nq):
+                got = o[b["starts"][i]:b["starts"][i + 1]]
+                want, _, A, mag = ac.ref_attend(b["queries"][i], *b["keys"][i], plan.scale, True)
+                ac.assert_attended("early rows", got[:n - 2], want[:n - 2], A[:n - 2], mag[:n - 2], n, 64, dt)
+                assert not torch.isfinite(got[n - 1]).all() and not torch.isfinite(got[n - 2, :, ::3]).any()
+
+
 def layer(plan, x, wqkv, pos, q_start):
     """One attention layer over packed tokens, as a user runs it."""
     H, Hk, D = plan.heads, plan.kv_heads, plan.head_dim
