@@ -148,8 +148,9 @@ class AttentionPlan(_Plan):
             _refuse(True, "pos: a contiguous int32 or float32 tensor [%d][%d] on %s", T, self.naxes, self.device)
         q_out, k_out = out if out is not None else (None, None)
         if q_out is None:
-            q_out = q.new_empty((T, H, D))
-        ldqo, hsqo = self._rows("q_out", q_out, H, dt, T)
+            q_out, ldqo, hsqo = q.new_empty((T, H, D)), H * D, D
+        else:
+            ldqo, hsqo = self._rows("q_out", q_out, H, dt, T)
         kp = vp = kop = vop = rowp = ldk = hsk = ldv = hsv = ldko = hsko = ldvo = hsvo = rows = 0
         if k is None:
             _refuse(v is not None or cache is not None or k_out is not None, "v, a cache and out[1] need k")
@@ -160,8 +161,9 @@ class AttentionPlan(_Plan):
                 _refuse(row is not None, "cache and row come together")
                 _refuse(v is not None, "v needs a cache")
                 if k_out is None:
-                    k_out = k.new_empty((T, Hk, D))
-                ldko, hsko = self._rows("k_out", k_out, Hk, dt, T)
+                    k_out, ldko, hsko = k.new_empty((T, Hk, D)), Hk * D, D
+                else:
+                    ldko, hsko = self._rows("k_out", k_out, Hk, dt, T)
             else:
                 _refuse(row is None, "cache and row come together")
                 _refuse(k_out is not None, "out[1] and a cache are one too many")
@@ -238,8 +240,7 @@ class AttentionPlan(_Plan):
             _refuse(True, "k has shape %s, v %s", tuple(k.shape), tuple(v.shape))
         lp = self._ints("k_len", k_len, B) if k_len is not None else 0
         if out is None:
-            out = q.new_empty((Tq, H, D))
-            ldo, hso = H * D, D
+            out, ldo, hso = q.new_empty((Tq, H, D)), H * D, D
         else:
             ldo, hso = self._rows("out", out, H, dt, Tq)
         logs = torch.empty((Tq, H), dtype=torch.float32, device=self.device) if lse else None

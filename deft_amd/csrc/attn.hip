@@ -507,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
 }
 
 template <int DT, int D, int NW>
-__global__ __launch_bounds__(64 * NW, D <= 64 ? 4 : 2) void attn_step_kernel(DeftAttn p, Grid grid) {
+__global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 64 ? 3 : 2) void attn_step_kernel(DeftAttn p, Grid grid) {
     typedef Tile<DT, D> TL;
     typedef typename TL::T T;
     // One wave: one stage -- twice the workgroups on a compute unit are worth more than the overlap (500 fp32 histories of up to 50: 20.5 us against

@@ -164,6 +164,8 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
             }
             T* const dst = isq ? (T*)p.q_out + (long long)t * p.ldqo + (long long)h * p.hsqo
                                : !isv ? (T*)p.k_out + krow * p.ldko + (long long)(h - p.Hq) * p.hsko : (T*)p.v_out + krow * p.ldvo + (long long)(h - Hqk) * p.hsvo;
+            // (non-temporal stores write 671 MB in 139 us instead of 144.5, but the attention behind them then reads q and k from memory: 5000 fp32
+            // tokens, both calls, 43 -> 57 us)
             *(vec*)(dst + lo) = a;
             *(vec*)(dst + hi) = b;
         }
