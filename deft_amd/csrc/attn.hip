@@ -13,7 +13,8 @@
 //
 // The reference M moves only when a score exceeds it by 2^8 (P <= 2^8 then, harmless in fp32 sums and in 16-bit P): the rescaling of O and the
 // exchange between the two half-waves of a row run on few tiles instead of on all.  fp16 keeps P at 2^6 times its value, so that small
-// probabilities stay out of the subnormals.
+// probabilities stay out of the subnormals.  16-bit types round each probability once for the matrix instruction (half a step relative, averaged over
+// the keys); their sum takes the unrounded ones.
 //
 // Two kernels:
 //   attn_prompt_kernel: 128 rows (4 waves x 32), key tiles shared by the waves, double-buffered in LDS by DMA.
@@ -68,7 +69,7 @@ __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? l
 
 // What a workgroup works on: sequence b, its query rows and keys, and the tile's rows.
 struct Work {
-    int b, hk, split;
+    int hk, split;
     int q0, n, m;                 // first query, queries, keys
     int row0, rows;               // first row of the tile, rows of the sequence (n * G)
     int qi, rem;                  // row0 = qi * G + rem
@@ -122,13 +123,13 @@ __device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, const Gr
             q1 = c >> 6 == i ? b : q1;
         }
     }
-    const int b = w.b = __builtin_amdgcn_readfirstlane(lo + c - 1);
+    const int b = __builtin_amdgcn_readfirstlane(lo + c - 1);
     w.q0 = __builtin_amdgcn_readfirstlane(q0);
     w.n = __builtin_amdgcn_readfirstlane(q1) - w.q0;
     if (w.n <= 0) return false;
     w.rows = w.n * G;
     const int tile = t - (w.q0 * G / BM + b);
-    if (tile >= (w.rows + BM - 1) / BM) return false;
+    if (tile < 0 || tile >= (w.rows + BM - 1) / BM) return false;                    // (negative: only where q_start does not grow)
     w.row0 = tile * BM;
     w.qi = G == 1 ? w.row0 : w.row0 / G;
     w.rem = w.row0 - w.qi * G;
@@ -652,7 +653,7 @@ int attn_check(const DeftAttn* d) {
     DEFT_CHECK(d->dtype == DEFT_F32 || d->dtype == DEFT_F16 || d->dtype == DEFT_BF16, -131, "deft_attn: dtype=%d", d->dtype);
     DEFT_CHECK(d->D == 32 || d->D == 64 || d->D == 96 || d->D == 128, -132, "deft_attn: D=%d (32, 64, 96 or 128)", d->D);
     DEFT_CHECK(d->Hk > 0 && d->Hq > 0 && d->Hq % d->Hk == 0 && d->Hq <= 4096, -133, "deft_attn: Hq=%d is not a multiple of Hk=%d", d->Hq, d->Hk);
-    DEFT_CHECK(d->Tq >= 0 && d->B >= 0 && d->slots >= 0 && d->cap >= 0, -134, "deft_attn: Tq=%d B=%d slots=%d cap=%d", d->Tq, d->B, d->slots, d->cap);
+    DEFT_CHECK(d->Tq >= 0 && d->B >= 0 && d->slots >= 0 && d->slots <= (1 << 30) && d->cap >= 0 && d->cap <= (1 << 30), -134, "deft_attn: Tq=%d B=%d slots=%d cap=%d", d->Tq, d->B, d->slots, d->cap);
     DEFT_CHECK((long long)d->Tq * d->Hq < (1ll << 30) && (long long)d->B * d->Hk < (1ll << 24), -134, "deft_attn: Tq=%d x Hq=%d rows, B=%d (below 2^30, 2^24 / Hk)", d->Tq, d->Hq, d->B);
     DEFT_CHECK(d->cap == 0 || (d->k_start && d->k_len), -135, "deft_attn: a cache (cap=%d) needs k_start (slots) and k_len", d->cap);
     const int V = d->dtype == DEFT_F32 ? 4 : 8;

@@ -111,6 +111,10 @@ def test_starts_and_lengths_are_clamped(emu_lib):
     o = plan.attend(q, kp, kp, i32(0, 2, 99), k_start=i32(13, 40), k_len=i32(50, 3))
     want = plan.attend(q[:2], kp, kp, i32(0, 2), k_start=i32(13), k_len=i32(2))
     assert torch.equal(o[:2], want) and (o[2:] == 0).all()
+    for bad in (i32(0, 4, 2, 4), i32(3, 1, 0, 4), i32(-7, 2, 99, 3), i32(4, 0, 4, 0)):      # starts that do not grow: some rows, but rows of q
+        o = plan.attend(q, kp, kp, bad, out=torch.full((4, 2, 32), 5.0))
+        assert torch.isfinite(o).all()
+        o = plan.attend(q, kp, kp, bad, k_start=i32(0, 9, 14), k_len=i32(15, 15, 15), max_k=700, out=torch.full((4, 2, 32), 5.0))
     assert (plan.attend(q, kp[:0], kp[:0], i32(0, 4)) == 0).all()              # no keys at all
     assert plan.attend(q[:0], kp, kp, i32(0)).shape == (0, 2, 32)
 
