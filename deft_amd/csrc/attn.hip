@@ -618,8 +618,8 @@ template <int DT>
 __global__ __launch_bounds__(256) void attn_merge_kernel(DeftAttn p, int nsplit) {
     typedef typename Elem<DT>::T T;
     const int lane = threadIdx.x & 63;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int q = (int)(row / p.Hq), h = (int)(row - (long long)q * p.Hq);
+    const unsigned row = blockIdx.x * 4 + (threadIdx.x >> 6);                      // (Tq * Hq < 2^30)
+    const int q = (int)(row / (unsigned)p.Hq), h = (int)(row - (unsigned)q * (unsigned)p.Hq);
     if (q >= p.Tq || q < p.q_start[0] || q >= p.q_start[p.B]) return;
     // lane s: M and L of split s (at most 64); then the splits' rows, whose loads wait for nothing
     const float2 x = lane < nsplit ? *(const float2*)(ws_ml(p, nsplit) + ws_row(p, lane, q, h) * 2) : make_float2(M_NONE, 0.f);
@@ -629,13 +629,25 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(DeftAttn p, int nsplit)
     float L = x.y * al, o0 = 0.f, o1 = 0.f;
     for (int i = 1; i < 64; i <<= 1) L += __shfl_xor(L, i);
     const int col = lane * 2 < p.D ? lane * 2 : 0;
-    for (unsigned long long some = deft_ballot(x.y != 0.f); some; some &= some - 1) {             // (splits that saw keys of this row)
-        const int s = __builtin_ctzll(some);
-        const float2 y = *(const float2*)(p.ws + ws_row(p, s, q, h) * p.D + col);
-        const float a = __shfl(al, s);
-        o0 = fmaf(y.x, a, o0);
-        o1 = fmaf(y.y, a, o1);
-    }
+    const unsigned long long some = deft_ballot(x.y != 0.f);                       // splits that saw keys of this row: the others have written no O
+    const int first = some ? __builtin_ctzll(some) : 0;
+    if (some)
+        for (int s0 = 0; s0 < nsplit; s0 += 8) {                                   // eight rows in flight
+            float2 y[8];
+            float a[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int s = (some >> ((s0 + i) & 63)) & 1 && s0 + i < 64 ? s0 + i : first;
+                y[i] = *(const float2*)(p.ws + ws_row(p, s, q, h) * p.D + col);
+                a[i] = __shfl(al, s);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool has = s0 + i < 64 && (some >> ((s0 + i) & 63)) & 1;
+                o0 = has ? fmaf(y[i].x, a[i], o0) : o0;
+                o1 = has ? fmaf(y[i].y, a[i], o1) : o1;
+            }
+        }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     if (lane * 2 < p.D) {
         T* const op = (T*)p.o + (long long)q * p.ldo + (long long)h * p.hso + lane * 2;
