@@ -17,6 +17,7 @@ template <> struct Elem<DEFT_BF16> { typedef __bf16 T; };
 
 constexpr int ROT_MAX_PAIRS = 128;
 constexpr int ROT_WAVES = 4;
+constexpr int ROT_ANGLES = 512;          // angles a wave holds: tokens of the wave x pairs <= 64 V (few heads) or ROT_MAX_PAIRS (one token)
 
 // sine and cosine of 2 pi r, r in turns: quarter turns leave in double, then |t| <= pi / 4 in fp32 (Taylor: the first dropped terms are
 // t^11 / 11! < 2e-9 and t^12 / 12! < 2e-10, below half an fp32 ulp of the results)
@@ -46,19 +47,22 @@ template <int S> __device__ __forceinline__ float deft_add_xor(float v) {
 __device__ __forceinline__ float deft_rsq(float x) { return __builtin_amdgcn_rsqf(x); }
 #endif
 
-// One wave: one token, `parts` waves sharing its heads.  LPH lanes a head (a power of two >= D / 2V; the surplus lanes of D = 96 idle).
+// One wave: one token, `parts` waves sharing its heads; or, where all heads of a token take a fraction of the lanes, several tokens (slots lanes' heads
+// each: 64 / LPH / slots tokens).  LPH lanes a head (a power of two >= D / 2V; the surplus lanes of D = 96 idle).
 // The heads of the next pass are fetched before those of this one are worked on, the first ones before the angles; norm weights stay in registers.
-template <int DT, bool ADJ, bool NORM, int LPH>
-__global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, int parts, float inv_d) {
+template <int DT, bool ADJ, bool NORM, int LPH, bool MANY>
+__global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, int parts, int slots_log2, float inv_d) {
     typedef typename Elem<DT>::T T;
     constexpr int V = 16 / (int)sizeof(T), HPW = 64 / LPH;
     typedef T vec __attribute__((ext_vector_type(V)));
-    __shared__ __attribute__((aligned(16))) float cs_s[ROT_WAVES][2][ROT_MAX_PAIRS];
+    __shared__ __attribute__((aligned(16))) float cs_s[ROT_WAVES][2][MANY ? ROT_ANGLES : ROT_MAX_PAIRS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned unit = blockIdx.x * ROT_WAVES + wave;                           // (T * parts < 2^31)
-    const int t = __builtin_amdgcn_readfirstlane((int)(parts == 1 ? unit : unit / (unsigned)parts)), part = __builtin_amdgcn_readfirstlane((int)(unit - (unsigned)t * (unsigned)parts));
-    const bool live = t < p.T;
-    const int c = lane & (LPH - 1), sub = lane / LPH;
+    const int c = lane & (LPH - 1), sub = lane / LPH, slots = MANY ? 1 << slots_log2 : HPW;
+    const int tokens = MANY ? HPW >> slots_log2 : 1, tok = MANY ? sub >> slots_log2 : 0;      // of this wave
+    const int wt = __builtin_amdgcn_readfirstlane((int)(parts == 1 ? unit : unit / (unsigned)parts)), part = __builtin_amdgcn_readfirstlane((int)(unit - (unsigned)wt * (unsigned)parts));
+    const int t0 = wt * tokens, t = t0 + tok;
+    const bool some = t0 < p.T, live = t < p.T;
     const bool mine = live && c < p.D / (2 * V);
     const bool turns = c * V < p.R;
     // this lane's two chunks; the pairs whose sines and cosines it needs are c V .. c V + V - 1
@@ -83,30 +87,38 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
             b = *(const vec*)(src + hi);
         }
     };
-    int h = part * HPW + sub;
+    int h = part * slots + (sub & (slots - 1));
     vec a, b;
     load(h, a, b);
     float* const cs_c = cs_s[wave][0];
     float* const cs_n = cs_s[wave][1];
-    if (live) {
-        for (int i = lane; i < p.R; i += 64) {
-            int ax = p.axis[i];
+    if (some) {
+        const int n = (p.T - t0 < tokens ? p.T - t0 : tokens) * p.R;
+        for (int i = lane; i < n; i += 64) {
+            const int k = tokens == 1 ? 0 : i / p.R, pair = i - k * p.R;
+            int ax = p.axis[pair];
             ax = ax < 0 ? 0 : (ax < p.A ? ax : p.A - 1);
-            const size_t at = (size_t)t * p.A + ax;
-            const double x = p.pos_float ? (double)((const float*)p.pos)[at] : (double)((const int*)p.pos)[at];
+            const size_t row = (size_t)(t0 + k) * p.A;
+            int raw[3];                                                            // (the usual axes wait for no table)
+#pragma unroll
+            for (int a = 0; a < 3; ++a) raw[a] = ((const int*)p.pos)[row + (a < p.A ? a : 0)];
+            int bits = ax == 0 ? raw[0] : ax == 1 ? raw[1] : raw[2];
+            if (ax > 2) bits = ((const int*)p.pos)[row + ax];
+            const double x = p.pos_float ? (double)__int_as_float(bits) : (double)bits;
             float sn, cs;
-            turn_sincos(x * p.freq[i] * 0.15915494309189535, sn, cs);
+            turn_sincos(x * p.freq[pair] * 0.15915494309189535, sn, cs);
             cs_c[i] = cs;
             cs_n[i] = p.inverse ? -sn : sn;
         }
     }
     __syncthreads();
-    if (!live) return;
+    if (!some) return;
+    const int at = tok * p.R + c * V;                                              // (rows behind T: values nobody uses, inside the array)
     float cv[V], sv[V], wq[2 * V], wk[2 * V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        cv[e] = turns ? cs_c[c * V + e] : 1.f;
-        sv[e] = turns ? cs_n[c * V + e] : 0.f;
+        cv[e] = turns && live ? cs_c[at + e] : 1.f;
+        sv[e] = turns && live ? cs_n[at + e] : 0.f;
     }
     if constexpr (NORM) {
 #pragma unroll
@@ -116,9 +128,9 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
             wk[e] = p.k_weight && mine ? p.k_weight[d] : 1.f;
         }
     }
-    for (int h0 = part * HPW; h0 < Hall; h0 += parts * HPW) {
+    for (int h0 = part * slots; h0 < Hall; h0 += parts * slots) {
         vec a2, b2;
-        load(h + parts * HPW, a2, b2);
+        load(h + parts * slots, a2, b2);
         const bool isq = h < p.Hq, isv = h >= Hqk;
         float x[V], y[V];
 #pragma unroll
@@ -171,7 +183,7 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
         }
         a = a2;
         b = b2;
-        h += parts * HPW;
+        h += parts * slots;
     }
 }
 
@@ -181,17 +193,22 @@ bool out_fits(long long ld, long long hs, int V, long long rows, int H, int D) {
     return in_fits(ld, hs, V) && (rows <= 1 || ld >= D) && (H <= 1 || hs >= D);
 }
 
-struct RotLaunch { unsigned grid; int parts; float inv_d; hipStream_t s; };
-template <int DT, int LPH>
-void rotary_launch(const DeftRotary& d, const RotLaunch& l) {
+struct RotLaunch { unsigned grid; int parts, slots_log2; float inv_d; hipStream_t s; };
+template <int DT, int LPH, bool MANY>
+void rotary_launch_k(const DeftRotary& d, const RotLaunch& l) {
     const dim3 g(l.grid), b(64 * ROT_WAVES);
     if (d.norm) {
-        if (d.adjacent) hipLaunchKernelGGL((rotary_kernel<DT, true, true, LPH>), g, b, 0, l.s, d, l.parts, l.inv_d);
-        else hipLaunchKernelGGL((rotary_kernel<DT, false, true, LPH>), g, b, 0, l.s, d, l.parts, l.inv_d);
+        if (d.adjacent) hipLaunchKernelGGL((rotary_kernel<DT, true, true, LPH, MANY>), g, b, 0, l.s, d, l.parts, l.slots_log2, l.inv_d);
+        else hipLaunchKernelGGL((rotary_kernel<DT, false, true, LPH, MANY>), g, b, 0, l.s, d, l.parts, l.slots_log2, l.inv_d);
     } else {
-        if (d.adjacent) hipLaunchKernelGGL((rotary_kernel<DT, true, false, LPH>), g, b, 0, l.s, d, l.parts, l.inv_d);
-        else hipLaunchKernelGGL((rotary_kernel<DT, false, false, LPH>), g, b, 0, l.s, d, l.parts, l.inv_d);
+        if (d.adjacent) hipLaunchKernelGGL((rotary_kernel<DT, true, false, LPH, MANY>), g, b, 0, l.s, d, l.parts, l.slots_log2, l.inv_d);
+        else hipLaunchKernelGGL((rotary_kernel<DT, false, false, LPH, MANY>), g, b, 0, l.s, d, l.parts, l.slots_log2, l.inv_d);
     }
+}
+template <int DT, int LPH>
+void rotary_launch(const DeftRotary& d, const RotLaunch& l) {
+    if ((64 / LPH) >> l.slots_log2 > 1) rotary_launch_k<DT, LPH, true>(d, l);
+    else rotary_launch_k<DT, LPH, false>(d, l);
 }
 template <int DT>
 void rotary_launch_lanes(const DeftRotary& d, const RotLaunch& l, int lanes) {
@@ -241,9 +258,14 @@ extern "C" int deft_rotary(const DeftRotary* d, void* stream) {
     // waves per token: one is the least angle work; few tokens take more, up to one pass each, until the chip's 256 x 16 waves are there
     int parts = 1;
     while (parts < passes && (long long)d->T * parts < 4096) ++parts;
-    const long long units = (long long)d->T * parts;
+    // tokens per wave: more than one where their heads fit, as long as 4096 waves remain (60000 tokens of 1 + 1 heads, D = 32: 28 -> 9 us; of 4 + 1, D = 64:
+    // 75 -> 46; a kernel of its own, since per-lane tokens cost the one-token form 7 %)
+    int slots_log2 = 0, tokens = 1;
+    while ((64 / lanes) >> slots_log2 > 1) ++slots_log2;
+    while (slots_log2 > 0 && heads <= 1 << (slots_log2 - 1) && d->T / (2 * tokens) >= 4096) { --slots_log2; tokens *= 2; }
+    const long long units = (long long)deft_cdiv(d->T, tokens) * parts;
     DEFT_CHECK(units < (1ll << 31), -123, "deft_rotary: T=%d", d->T);
-    const RotLaunch l = {(unsigned)((units + ROT_WAVES - 1) / ROT_WAVES), parts, 1.f / (float)d->D, (hipStream_t)stream};
+    const RotLaunch l = {(unsigned)((units + ROT_WAVES - 1) / ROT_WAVES), parts, slots_log2, 1.f / (float)d->D, (hipStream_t)stream};
     if (d->dtype == DEFT_F32) rotary_launch_lanes<DEFT_F32>(*d, l, lanes);
     else if (d->dtype == DEFT_F16) rotary_launch_lanes<DEFT_F16>(*d, l, lanes);
     else rotary_launch_lanes<DEFT_BF16>(*d, l, lanes);

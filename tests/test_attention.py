@@ -21,6 +21,9 @@ F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
     dict(T=5, H=5, Hk=1, D=64, axes=(16, 16), inplace=True),
     dict(T=5, H=5, Hk=1, D=64, axes=(16, 16), norm=True, inplace=True, adjacent=True),
     dict(T=2, H=6, Hk=1, D=64, axes=(8,), k_none=True),
+    dict(T=8201, H=1, Hk=1, D=32, axes=(8, 8), norm=True),                    # several tokens a wave, an odd count of them
+    dict(T=16390, H=1, Hk=1, D=32, axes=(4, 4), adjacent=True, cache="rows"),
+    dict(T=8195, H=2, Hk=1, D=96, axes=(24, 16), k_none=True),
 ])
 def test_rotary(emu_lib, dt, kw):
     ac.check_rotary(emu_lib, "cpu", dt, **kw)

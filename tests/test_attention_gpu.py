@@ -20,6 +20,8 @@ F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
     dict(T=1, H=40, Hk=8, D=128, axes=(16, 24, 24), norm=True, weights=False),
     dict(T=61, H=2, Hk=2, D=256, axes=(64, 32, 32), far=True, inverse=True),
     dict(T=5001, H=5, Hk=1, D=64, axes=(16, 16), norm=True, inplace=True),
+    dict(T=33001, H=1, Hk=1, D=32, axes=(8, 8), norm=True, cache="rows"),      # several tokens a wave, an odd count of them
+    dict(T=9001, H=3, Hk=1, D=64, axes=(16, 16), adjacent=True),
 ])
 def test_rotary(gpu_lib, dt, kw):
     ac.check_rotary(gpu_lib, "cuda", dt, **kw)
