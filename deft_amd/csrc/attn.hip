@@ -21,6 +21,10 @@
 //   attn_step_kernel:   32 rows, the waves take different key tiles, each with its own double-buffered LDS, joined at the end: single tokens
 //                       over long histories, where the keys' bytes are the cost.
 // Both can split the keys over workgroups (partial O, M, L in the workspace, attn_merge_kernel joins them in order).
+//
+// Measured (one MI355X, a call among others): one 16384-token sequence, 16 heads over 4 of 128, bf16, causal: 1.01 - 1.05 ms, 1050 - 1090 TFLOP/s -- MFMA busy
+// 59 % and VALU 51 % of the cycles, the two of them share the clock the card holds; D = 64: 905 TFLOP/s (8 heads, 16384), VALU-bound (an exponential is
+// a quarter-rate instruction a score); 24 single tokens over 2000 .. 32000 keys, 32 heads over 8 of 128, bf16: 359 us, 5.25 TB/s of keys and values.
 #include "common.h"
 
 namespace {

@@ -6,6 +6,8 @@
 // rotation needs no exchange between lanes and the norm one butterfly over the D / (2 V) lanes of a head (V = elements of 16 bytes).  The
 // angles depend on the token alone: a wave forms its token's R sines and cosines once (in double up to the quarter turn, then two short
 // polynomials) and keeps the 2 V values of its lane's chunks in registers for all heads it handles.
+// Measured (one MI355X, cold inputs): 32781 tokens of 32 + 8 heads of 128, bf16, norm and rotation: 145 us, 4.65 TB/s (a large copy: 5.1); 100 fp32
+// tokens of 8 + 8 heads of 32: 4.1 us on the device.
 #include "common.h"
 
 namespace {
