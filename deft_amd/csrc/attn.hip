@@ -687,6 +687,8 @@ struct Choice { bool step; int waves, nsplit, ntiles; };
 Choice choose(const DeftAttn* d) {
     const int G = d->Hq / d->Hk;
     Choice c;
+    // 32-row tiles where sequences have no more rows, or one or two key tiles (200 histories of up to 50, 4 heads a group: 12.6 us against 14.4 with
+    // 128-row tiles; 100 of 40 .. 120: 68 against 17; 4000 x 4000, D = 128: 186 against 70)
     c.step = (long long)d->Tq * G <= 32ll * d->B || d->max_k <= 64;
     const int bm = c.step ? 32 : BM;
     c.ntiles = d->Tq * G / bm + d->B;                              // (below 2^26 + 2^24)
@@ -697,6 +699,8 @@ Choice choose(const DeftAttn* d) {
     // one wave a row tile where the keys are one or two tiles, or where that already fills the chip (256 x 8 heads over 100 .. 500 keys, D = 128: 71 us
     // against 92 with four; 200 x 4 over 30 .. 120: 10.1 against 12.3; 256 x 4 over 500, D = 64: 22 against 21)
     c.waves = c.step && (d->max_k <= 64 || (busy >= 800 && d->max_k <= 512)) ? 1 : 4;
+    // key pieces: step kernel up to 2048 workgroups (24 x 32000 keys: 360 us; up to 1024: 373, 4096: 369), prompt kernel 768 (300-token chunks: 42.7 us; 512:
+    // 44.0, 1024: 46.8; 4000 x 4000: 58.9, 70, 76.9); pieces of 256 keys instead of 512 help fp32 (194 -> 182 us on chunks) and not the others (42.6 -> 48.7)
     long long want = (c.step ? 2048 : 768) / busy;
     const long long most = ((long long)d->max_k + keys - 1) / keys;
     if (want > most) want = most;

@@ -206,3 +206,34 @@ def test_packed_descriptors_match_the_mirrors():
         vals = [i + 1 for i in range(len(mirror._fields_) - 1)] + [0.5]
         d = mirror.from_buffer_copy(fmt.pack(*vals))
         assert [getattr(d, n) for n, _ in mirror._fields_] == vals
+
+
+def test_lds_fetches_keep_their_wait_states(tmp_path):
+    """csrc/attn.hip writes its LDS-DMA out in assembly, where the compiler inserts no wait states: a scalar register that a vector instruction has written
+    may be a memory instruction's source only five states later, and m0 one state after its write.  Checked on every one of the built code."""
+    import os
+    import re
+    import subprocess
+    from deft_amd import build
+    build.build(force=False, verbose=False)
+    llvm = "/opt/rocm/lib/llvm/bin/"
+    if not os.path.exists(llvm + "llvm-objdump"):
+        pytest.skip("llvm-objdump not in this image")
+    fat, co = str(tmp_path / "fat.bin"), str(tmp_path / "dev.co")
+    subprocess.check_call([llvm + "llvm-objcopy", "-O", "binary", "--only-section=.hip_fatbin", os.path.join(build.OBJ_DIR, "attn.hip.o"), fat])
+    subprocess.check_call([llvm + "clang-offload-bundler", "--unbundle", "--type=o", "--input=" + fat, "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", "--output=" + co])
+    code = [ln.split("//")[0].strip() for ln in subprocess.run([llvm + "llvm-objdump", "-d", co], capture_output=True, text=True).stdout.splitlines()]
+    fetches = 0
+    for i, ins in enumerate(code):
+        m = re.match(r"buffer_load_dwordx4 v\d+, s\[(\d+):(\d+)\].* lds", ins)
+        if not m:
+            continue
+        fetches += 1
+        assert code[i - 1].startswith("s_nop") and code[i - 2].startswith("s_mov_b32 m0"), code[i - 3:i + 1]
+        source, states, j = range(int(m[1]), int(m[2]) + 1), 0, i - 1
+        while states < 5:
+            w = re.match(r"v_read(?:first)?lane_b32 s(\d+)", code[j])
+            assert not w or int(w[1]) not in source, code[j:i + 1]
+            states += 1 + int(code[j].split()[1]) if code[j].startswith("s_nop") else 1
+            j -= 1
+    assert fetches > 100
