@@ -216,9 +216,8 @@ SPLITK = _os.environ.get("DEFT_SPLITK", "1") != "0"
 # launch lists of at most DATAFLOW_MAX_N frames CAN run over this many HIP streams along their data dependencies (_Plan.build_schedule): one
 # frame per GPU leaves most of the chip idle in most launches, and DLA-34's up path has independent branches -- captured as a hipGraph that is a
 # graph with two parallel branches, 1.77 instead of 2.00 ms per frame in the one-frame latency mode.  OFF by default since round 6 (one stream,
-# one branch): ROCm 7.2's hipGraphLaunch walks off the end of an executable graph's internal stream list for graphs WITH parallel branches after
-# certain process histories (hip::Graph::UpdateStreams, a host segfault; profiles/r6_graph_replay_segfault.md -- moving the launch to another
-# stream does not avoid it).  DEFT_DATAFLOW=2 opts back in.
+# one branch): with ROCm 7.2 the replay of a graph WITH parallel branches has ended in a host segmentation fault after certain process histories
+# (profiles/r6_graph_replay_segfault.md -- moving the launch to another stream does not avoid it).  DEFT_DATAFLOW=2 opts back in.
 DATAFLOW = int(_os.environ.get("DEFT_DATAFLOW", "1"))
 DATAFLOW_MAX_N = int(_os.environ.get("DEFT_DATAFLOW_MAX_N", "1"))
 REPLAY_STREAM = _os.environ.get("DEFT_REPLAY_STREAM", "0") != "0"      # 1: a hipGraph replay that would land on the NULL stream runs on a side stream (experiment)

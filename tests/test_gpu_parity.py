@@ -792,9 +792,8 @@ def test_graph_replay_survives_tracker_teardown(gpu_lib):
 
 
 def test_captured_graphs_have_no_parallel_branch_by_default(gpu_lib):
-    """ROCm 7.2's hipGraphLaunch of a graph WITH parallel branches walks off the end of the executable graph's internal stream list after
-    certain process histories (hip::Graph::UpdateStreams: a host segfault; profiles/r6_graph_replay_segfault.md, reproducer
-    tools/probe/r6_crash_fix.sh).  The package therefore captures its launch lists on ONE stream unless DEFT_DATAFLOW=2 asks for the two-branch
+    """With ROCm 7.2 the replay of a graph WITH parallel branches has ended in a host segmentation fault after certain process histories
+    (profiles/r6_graph_replay_segfault.md).  The package therefore captures its launch lists on ONE stream unless DEFT_DATAFLOW=2 asks for the two-branch
     schedule: a serial Detector.run loop captures a plan without a schedule, and its results are what the eager launch list gives."""
     from types import SimpleNamespace
     from deft_amd import engine
