@@ -3,12 +3,11 @@
 mkdir -p gpurun_out/r5b
 O=gpurun_out/r5b
 ./tools/probe/f16_denorm.bin > $O/f16_denorm.log 2>&1
-timeout 120 ./tools/probe/pkf32_min.bin 20 > $O/pkf32_min.log 2>&1
 timeout 900 python -m pytest tests/test_gpu_parity.py -q --maxfail=12 -k "not seed_sweep" --durations=25 > $O/pytest_np2.log 2>&1
 for lib in hip bf16x3; do
   DEFT_HIP_LIB=$PWD/deft_amd/lib/libdeft_$lib.so timeout 300 python bench.py --steps 20 --warmup 5 --no-extras --no-cpu-baseline > $O/bench_$lib.json 2> $O/bench_$lib.err
 done
-tail -4 $O/pytest_np2.log; cat $O/f16_denorm.log; tail -3 $O/pkf32_min.log
+tail -4 $O/pytest_np2.log; cat $O/f16_denorm.log
 python - <<'PY'
 import json
 for lib in ("hip", "bf16x3"):
