@@ -81,7 +81,7 @@ class AttentionPlan(_Plan):
             ld, hs, one = x.stride()
             if h == heads and D == self.head_dim and x.dtype is dtype and one == 1 and (tokens is None or T == tokens) and x.get_device() == self._index \
                     and not x.requires_grad:
-                return 0 if T == 1 else ld, 0 if h == 1 else hs          # (the stride of a one-long dimension says nothing)
+                return D if T == 1 else ld, D if h == 1 else hs          # (the stride of a one-long dimension says nothing)
         except (AttributeError, ValueError, TypeError):
             pass
         return self._not_rows(name, x, heads, dtype, tokens, "[tokens]")
@@ -92,7 +92,7 @@ class AttentionPlan(_Plan):
             S, cap, h, D = x.shape
             ss, ld, hs, one = x.stride()
             if h == self.kv_heads and D == self.head_dim and x.dtype is dtype and one == 1 and x.get_device() == self._index and not x.requires_grad:
-                return 0 if S == 1 else ss, 0 if cap == 1 else ld, 0 if h == 1 else hs
+                return 0 if S == 1 else ss, D if cap == 1 else ld, D if h == 1 else hs
         except (AttributeError, ValueError, TypeError):
             pass
         return self._not_rows(name, x, self.kv_heads, dtype, None, "[slots][rows]")

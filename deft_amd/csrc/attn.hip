@@ -147,6 +147,10 @@ __device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, const Gr
     w.v = (const char*)p.v + (vo + (long long)w.hk * p.hsv) * tsize;
     return true;
 }
+// Value rows of a tile in front of this key may hold something a row must not see: rows >= m arrive as zeros (Fetch::issue), unless rows share memory
+// (a stride below a row: expanded or sliding keys) -- then the range of the source does not end with row m - 1.
+template <int D>
+__device__ __forceinline__ int values_end(const DeftAttn& p, const Work& w) { return p.ldv < D ? 0x7fffffff : w.m; }
 // keys (j < vis) that query i of the sequence sees
 __device__ __forceinline__ int visible(const DeftAttn& p, const Work& w, int i) { return p.causal ? clampi(w.m - w.n + i + 1, 0, w.m) : w.m; }
 
@@ -181,7 +185,7 @@ struct Tile {
                 off[i] = (unsigned)(r * (int)ld) * (unsigned)TS + (unsigned)c * 16u;      // (ld <= 2^22, r < 64: below 2^31)
             }
         }
-        // rows >= nv arrive as zeros: the range of the source ends with row nv - 1
+        // rows >= nv arrive as zeros: the range of the source ends with row nv - 1 (rows closer than a row: see values_end)
         __device__ __forceinline__ void issue(const char* base, lds_at lds, int first, int by, int nv, int row_bytes) const {
             const lds_src r = lds_source(base, nv <= 0 ? 0u : nv >= 64 ? 0x7FFFFFFFu : (unsigned)((nv - 1) * row_bytes + RB));
 #pragma unroll
@@ -469,7 +473,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
     const int head = w.hk * G + w.rem + rc - (qi - w.qi) * G;
     const int vis = visible(p, w, qi);
     const int vmin = visible(p, w, query_of(wr0)), vmax = visible(p, w, query_of(wr0 + 31));                  // the wave's first and last row
-    const int bmax = visible(p, w, query_of(BM - 1));
+    const int bmax = visible(p, w, query_of(BM - 1)), vend = values_end<D>(p, w);
     const int nt = (bmax + BN - 1) / BN, per = split_tiles(grid, nt);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
@@ -494,12 +498,12 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
         const int k0 = t * BN;
         const char* const ks = lds + st * 2 * KB;
         if (on && k0 < vmax) {
-            const int end = k0 + BN < w.m ? k0 + BN : w.m;
+            const int end = k0 + BN < vend ? k0 + BN : vend;
             if (TL::template step<NT, false>(rw, ks, ks + KB, vis - k0, vmin < k0 + BN, vmin < end, sc, lane)) again = 1;
         }
     }
     __syncthreads();
-    if (p.causal && again) {                                                       // (rare: infinities or NaN behind the diagonal of some row)
+    if (again) {                                                                   // (rare: infinities or NaN behind the diagonal of some row)
         rw.clear();
         for (int t = t0; t < t1; ++t) {
             issue(t, 0);
@@ -529,7 +533,7 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
     const int left = w.rows - w.row0 - 1;                                          // the tile's last row
     auto query_of = [&](int r) { return w.qi + div_small(w.rem + (r < left ? r : left), grid.inv_g); };      // of row r of the tile (the last one's behind it)
     const int rc = l32 < left ? l32 : left, qi = query_of(rc), query = w.q0 + qi, head = w.hk * G + w.rem + rc - (qi - w.qi) * G;
-    const int vis = visible(p, w, qi), vmin = visible(p, w, w.qi), vmax = visible(p, w, query_of(31));
+    const int vis = visible(p, w, qi), vmin = visible(p, w, w.qi), vmax = visible(p, w, query_of(31)), vend = values_end<D>(p, w);
     const int nt = (vmax + 31) >> 5, per = split_tiles(grid, nt);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
@@ -551,7 +555,7 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
     if (NS == 2 && t0 + wave + NW < t1) issue(t0 + wave + NW, 1);
     for (int t = t0 + wave; t < t1; t += NW, st ^= NS - 1) {
         if (NS == 2 && t + NW < t1) { DEFT_WAVE_VM(2 * NI); } else { DEFT_WAVE_VM(0); }       // this wave's tile t is here (the stages are its own: no barrier)
-        const int k0 = t * 32, end = k0 + 32 < w.m ? k0 + 32 : w.m;
+        const int k0 = t * 32, end = k0 + 32 < vend ? k0 + 32 : vend;
         if (TL::template step<1, false>(rw, mine + st * 2 * KB, mine + st * 2 * KB + KB, vis - k0, vmin < k0 + 32, vmin < end, sc, lane)) again = 1;
         if (t + NS * NW < t1) {
             DEFT_WAVE_LGKM();                                                      // its reads have returned: the stage may be filled again

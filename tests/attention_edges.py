@@ -1,0 +1,39 @@
+"""Corners of deft_amd.attention, shared by the CPU (SIMT emulator) and the GPU tests.  References in 64 bits and tolerances: attention_checks.py."""
+import torch
+
+import attention_checks as ac
+from deft_amd.attention import AttentionPlan
+
+
+def i32(device, *x):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+def check_shared_key_rows(lib, device, dt, bad):
+    """Key rows behind the last one are never used, also where the stride between rows is shorter than a row (one key, a cache of one row, expanded or
+    sliding keys): an infinite or NaN value that IS visible comes back as it stands in the formula, not as 0 * inf of a row that is not there."""
+    g = torch.Generator().manual_seed(3)
+    D = 32
+    plan = AttentionPlan(2, 1, D, device=device, lib=lib)
+    q, k, v = ac.rand(g, dt, 5, 2, D).to(device), ac.rand(g, dt, 1, 1, D).to(device), ac.rand(g, dt, 1, 1, D).to(device)
+    v[0, 0, 3] = bad
+
+    def check(name, o, nq, keys, values, causal=True):
+        want, _, A, mag = ac.ref_attend(q[:nq].cpu(), keys.cpu(), values.cpu(), plan.scale, causal)
+        ac.assert_attended(name, o, want, A, mag, keys.shape[0], D, dt)
+
+    check("one key", plan.attend(q[:1], k, v, i32(device, 0, 1)), 1, k, v)
+    check("one key, not causal", plan.attend(q, k, v, i32(device, 0, 5), k_start=i32(device, 0), k_len=i32(device, 1), causal=False), 5, k, v, False)
+    one = (i32(device, 0), i32(device, 1))
+    check("cache of one row", plan.attend(q[:1], k[None], v[None], i32(device, 0, 1), slot=one[0], k_len=one[1]), 1, k, v)
+    for causal in (True, False):
+        ke, ve = k.expand(5, 1, D), v.expand(5, 1, D)
+        check("expanded", plan.attend(q, ke, ve, i32(device, 0, 5), causal=causal), 5, ke, ve, causal)
+    step = 16                                                        # rows that overlap: row r starts 16 elements behind row r - 1
+    flat = ac.rand(g, dt, 5 * step + D).to(device)
+    flat[4 * step + D - 1] = bad                                     # the last element of the last row of 5
+    flat[4 * step + D] = float("nan")                                # what a sixth row would hold
+    vs = flat.as_strided((5, 1, D), (step, step, 1))
+    k5 = ac.rand(g, dt, 5, 1, D).to(device)
+    for causal in (True, False):
+        check("sliding", plan.attend(q, k5, vs, i32(device, 0, 5), causal=causal), 5, k5, vs, causal)

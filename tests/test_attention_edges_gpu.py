@@ -1,0 +1,14 @@
+"""-m gpu: corners of the attention-layer operators on a real MI355X; the checks themselves are in tests/attention_edges.py."""
+import pytest
+import torch
+
+import attention_edges as ae
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_key_rows_that_share_memory(gpu_lib, dt, bad):
+    ae.check_shared_key_rows(gpu_lib, "cuda", dt, bad)
