@@ -156,7 +156,8 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
         }
         if (mine && h < Hall && (isq || kput)) {
             if (!isv) {
-                if constexpr (ADJ) {
+                if (!turns) {                                                      // (by its lanes: 1 * x - 0 * y is not x beside an infinity)
+                } else if constexpr (ADJ) {
 #pragma unroll
                     for (int e = 0; e < V; e += 2) {
                         const float x0 = x[e], x1 = x[e + 1], y0 = y[e], y1 = y[e + 1];

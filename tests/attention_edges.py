@@ -37,3 +37,21 @@ def check_shared_key_rows(lib, device, dt, bad):
     k5 = ac.rand(g, dt, 5, 1, D).to(device)
     for causal in (True, False):
         check("sliding", plan.attend(q, k5, vs, i32(device, 0, 5), causal=causal), 5, k5, vs, causal)
+
+
+def check_unturned_elements(lib, device, dt, adjacent, norm):
+    """Elements behind the 2 R first: as they were (normed where asked), whatever an element beside them holds."""
+    g = torch.Generator().manual_seed(5)
+    T, H, D, R = 7, 3, 64, 8
+    q = ac.rand(g, dt, T, H, D)
+    q[1, 0, 2 * R + 3], q[2, 1, D - 1], q[4, 2, D // 2 + 1] = float("inf"), float("-inf"), float("nan")
+    pos = torch.arange(T, dtype=torch.int32).view(T, 1)
+    plan = AttentionPlan(H, 1, D, axes=(R,), adjacent=adjacent, device=device, lib=lib)
+    got, _ = (plan.norm_rotate if norm else plan.rotate)(q.to(device), None, pos.to(device))
+    want, mag = ac.ref_rotate(q, pos, [10000.0 ** (-i / R) for i in range(R)], [0] * R, adjacent, norm=norm)
+    got = got.cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    if not norm:
+        assert torch.equal(torch.nan_to_num(got[..., 2 * R:], 7.0), torch.nan_to_num(q[..., 2 * R:], 7.0))
+    fine = torch.isfinite(want)
+    ac.assert_rotated("finite", got[fine], want[fine], torch.nan_to_num(mag, 0, 0, 0)[fine], dt)

@@ -12,3 +12,10 @@ F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
 def test_key_rows_that_share_memory(gpu_lib, dt, bad):
     ae.check_shared_key_rows(gpu_lib, "cuda", dt, bad)
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("adjacent", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_unturned_elements(gpu_lib, dt, adjacent, norm):
+    ae.check_unturned_elements(gpu_lib, "cuda", dt, adjacent, norm)
