@@ -47,7 +47,17 @@ template <int S> __device__ __forceinline__ float deft_add_xor(float v) {
     else return v + __shfl_xor(v, S);
 }
 __device__ __forceinline__ float deft_rsq(float x) { return __builtin_amdgcn_rsqf(x); }
+__device__ __forceinline__ unsigned long long deft_ballot(bool b) { return __ballot(b); }
 #endif
+// sum over the LPH lanes of a head
+template <int LPH> __device__ __forceinline__ float head_sum(float v) {
+    if constexpr (LPH > 1) v = deft_add_xor<1>(v);
+    if constexpr (LPH > 2) v = deft_add_xor<2>(v);
+    if constexpr (LPH > 4) v = deft_add_xor<4>(v);
+    if constexpr (LPH > 8) v = deft_add_xor<8>(v);
+    if constexpr (LPH > 16) v = deft_add_xor<16>(v);
+    return v;
+}
 
 // One wave: one token, `parts` waves sharing its heads; or, where all heads of a token take a fraction of the lanes, several tokens (slots lanes' heads
 // each: 64 / LPH / slots tokens).  LPH lanes a head (a power of two >= D / 2V; the surplus lanes of D = 96 idle).
@@ -141,13 +151,30 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
             float ss = 0.f;
 #pragma unroll
             for (int e = 0; e < V; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
-            if constexpr (LPH > 1) ss = deft_add_xor<1>(ss);
-            if constexpr (LPH > 2) ss = deft_add_xor<2>(ss);
-            if constexpr (LPH > 4) ss = deft_add_xor<4>(ss);
-            if constexpr (LPH > 8) ss = deft_add_xor<8>(ss);
-            if constexpr (LPH > 16) ss = deft_add_xor<16>(ss);
+            ss = head_sum<LPH>(ss);
             const float m = fmaf(ss, inv_d, p.eps);
-            const float r = m >= 1e-30f ? deft_rsq(m) : 1.f / sqrtf(m);            // (the hardware's root takes no subnormal)
+            float r = deft_rsq(m);
+            // squares that leave fp32 (or a mean near its end, where the hardware's root takes no subnormal): the head is brought to about 1 by a power
+            // of two first
+            const bool far = mine && h < Hqk && !(m >= 1e-30f && ss <= 1e37f);
+            if (deft_ballot(far) != 0) {
+                float top = sqrtf(p.eps);
+#pragma unroll
+                for (int e = 0; e < V; ++e) top = fmaxf(top, fmaxf(fabsf(x[e]), fabsf(y[e])));
+#pragma unroll
+                for (int s = 1; s < LPH; s <<= 1) top = fmaxf(top, __shfl_xor(top, s));
+                const int up = 254 - ((__float_as_int(top) >> 23) & 255);
+                const float by = far ? __int_as_float((up < 1 ? 1 : up > 253 ? 253 : up) << 23) : 1.f;
+                ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[e] *= by;
+                    y[e] *= by;
+                    ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
+                }
+                ss = head_sum<LPH>(ss);
+                r = far ? 1.f / sqrtf(fmaf(ss, inv_d, p.eps * by * by)) : r;
+            }
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 x[e] *= r * (isq ? wq[e] : wk[e]);

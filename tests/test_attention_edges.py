@@ -18,3 +18,9 @@ def test_key_rows_that_share_memory(emu_lib, dt, bad):
 @pytest.mark.parametrize("norm", [False, True])
 def test_unturned_elements(emu_lib, dt, adjacent, norm):
     ae.check_unturned_elements(emu_lib, "cpu", dt, adjacent, norm)
+
+
+@pytest.mark.parametrize("dt,size,eps", [(F32, 1e25, 1e-6), (BF16, 1e30, 1e-6), (F32, 3e37, 0.0), (F32, 1e-25, 0.0), (BF16, 1e-30, 0.0), (F32, 1e-20, 1e-38), (F16, 1e-5, 0.0),
+                                         (F32, 1e-30, 1e-6), (BF16, 1e19, 1e-6)])
+def test_norm_of_far_values(emu_lib, dt, size, eps):
+    ae.check_norm_of_far_values(emu_lib, "cpu", dt, size, eps)
