@@ -66,8 +66,13 @@ template <> struct Elem<DEFT_F16> { typedef _Float16 T; };
 template <> struct Elem<DEFT_BF16> { typedef __bf16 T; };
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float M_NONE = -3.0e38f;            // M of a row that has seen no key (finite: -inf - M must not become NaN)
 constexpr float M_SLACK = 8.f;
+// The reference M of a row starts at -2^24 and is good up to 2^24 (in log2): there s sc - M is one fma, and what M's own rounding takes off, the same for
+// every key of the row, is at most a factor of two.  A row whose scores lie beyond, on either side, has its pass run again with FAR, where scores are
+// rounded before the difference is taken and kept in HALF log2 units: a finite score then has a finite exponent whatever its size.  M leaves every
+// pass in half units (L = 0: M_LEAST).
+constexpr float M_NONE = -16777216.f, M_FAR = 16777216.f, M_LEAST = -3.4028234664e38f;
+enum { BAD_VALUES = 1, FAR = 2 };             // why a pass is run again
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
@@ -212,21 +217,23 @@ struct Tile {
     struct Rows {
         frag_t q[NF];                 // chunk 2 j + (l >> 5) of the row
         f32x16 o[NJ];                 // o[j][r]: column 32 j + 8 (r >> 2) + 4 (l >> 5) + (r & 3)
-        float M, L;                   // scores are kept times scale * log2 e; P = 2^(s - M); L: this half-wave's part
+        float M, L;                   // scores are taken times scale * log2 e; P = 2^(s - M); L: this half-wave's part
         __device__ __forceinline__ void init(const T* qrow, int h) {
 #pragma unroll
             for (int j = 0; j < NF; ++j) q[j] = *(const frag_t*)((const char*)qrow + (2 * j + h) * 16);
-            clear();
+            clear(M_NONE);
             // (the loads end here: a wait for them inside the loop would wait for the tiles fetched ahead)
 #pragma unroll
             for (int j = 0; j < NF; ++j) DEFT_OPAQUE(q[j]);
         }
-        __device__ __forceinline__ void clear() {
+        __device__ __forceinline__ void clear(float m) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) o[j] = zero16();
-            M = M_NONE;
+            M = m;
             L = 0.f;
         }
+        // whether some row (that saw keys: `saw`) has scores the reference could not follow down to; NaN stays NaN
+        __device__ __forceinline__ bool missed(bool saw) const { return deft_ballot(saw && M == M_NONE && L == L) != 0; }
     };
 
     // Any infinity or NaN among the BN rows of V?
@@ -246,9 +253,12 @@ struct Tile {
     }
     // One tile of BN = 32 NT keys for a wave: ks, vs the tile in LDS; vis: keys of the tile this lane's row sees (may be <= 0 or > BN); `partial`
     // (wave-uniform): some row does not see all of them; `hidden`: some row does not see keys that are there (their values must not reach it).
-    // Returns whether such hidden values are infinite or NaN: the wave's result is not valid then, and its pass is run again with CAREFUL.
+    // Returns whether such hidden values are infinite or NaN (BAD_VALUES) and whether a score is beyond M_FAR (FAR): the wave's result is not valid then,
+    // and its pass is run again with CAREFUL -- with the same exponentials, or, `far`, in half log2 units (sc: scale * log2 e, or half of that).
     template <int NT, bool CAREFUL>
-    static __device__ __forceinline__ bool step(Rows& w, const char* ks, const char* vs, int vis, bool partial, bool hidden, float sc, int lane) {
+    static __device__ __forceinline__ int step(Rows& w, const char* ks, const char* vs, int vis, bool partial, bool hidden, float sc, int lane, bool far = false) {
+        const bool half = CAREFUL && far;
+        const float first = half ? sc : 1.f, then = half ? 1.f : sc, units = half ? 2.f : 1.f;       // (products with 1 change nothing)
         const int h = lane >> 5;
         f32x16 s[NT];
         {
@@ -273,11 +283,16 @@ struct Tile {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
-        if (deft_ballot(mx * sc > w.M + (SHIFT + M_SLACK)) != 0) {
+            for (int r = 0; r < 16; ++r) {
+                if constexpr (CAREFUL) s[t][r] *= first;
+                mx = t + r == 0 ? s[0][0] : fmaxf(mx, s[t][r]);
+            }
+        int bad = 0;
+        if (deft_ballot(half ? (mx - w.M) * 2.f > SHIFT + M_SLACK : mx * sc > w.M + (SHIFT + M_SLACK)) != 0) {
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float Mn = fmaxf(w.M, mx * sc - SHIFT);
-            const float al = deft_exp2(w.M - Mn);
+            const float Mn = fmaxf(w.M, half ? mx - SHIFT * 0.5f : mx * sc - SHIFT);
+            const float al = deft_exp2(half ? (w.M - Mn) * 2.f : w.M - Mn);
+            if constexpr (!CAREFUL) bad = deft_ballot(Mn > M_FAR) != 0 ? FAR : 0;
             w.M = Mn;
             w.L *= al;
 #pragma unroll
@@ -290,14 +305,14 @@ struct Tile {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float e = deft_exp2(fmaf(s[t][r], sc, -w.M));
+                const float e = deft_exp2(CAREFUL ? fmaf(s[t][r], then, -w.M) * units : fmaf(s[t][r], sc, -w.M));
                 s[t][r] = e;
                 sum[r & 3] += e;
             }
         w.L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if constexpr (CAREFUL) {
             careful<NT>(w, s, vs, vis, lane);
-            return false;
+            return 0;
         } else {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -307,7 +322,7 @@ struct Tile {
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) w.o[j] = pv(value(vs, t, g, j, lane), pb, w.o[j]);
                 }
-            return hidden && any_bad<32 * NT>(vs, lane);
+            return hidden && any_bad<32 * NT>(vs, lane) ? bad | BAD_VALUES : bad;
         }
     }
 
@@ -399,6 +414,9 @@ __device__ __forceinline__ int split_tiles(const Grid& g, int nt) {
 __device__ __forceinline__ size_t ws_row(const DeftAttn& p, int split, int query, int head) { return ((size_t)split * p.Tq + query) * p.Hq + head; }
 __device__ __forceinline__ float* ws_ml(const DeftAttn& p, int nsplit) { return p.ws + (size_t)nsplit * p.Tq * p.Hq * p.D; }
 
+// the log of a row's sum of exponentials from its M (half units) and L
+__device__ __forceinline__ float log_sum(float M, float L) { return L == 0.f ? -INFINITY : (M + deft_log2(L) * 0.5f) * (2.f * LN2); }
+
 // A wave's 32 rows to the output, or to the workspace where the keys are split: through its part of the LDS stages (32 rows, chunks swizzled like
 // K's), so that rows leave as whole lines -- in the accumulators a lane holds 4 of every 8 columns of one row.
 template <int DT, int D>
@@ -407,6 +425,7 @@ __device__ __forceinline__ void write_rows(const DeftAttn& p, const Work& w, typ
     typedef typename TL::T T;
     const int h = lane >> 5, l32 = lane & 31;
     rw.L += __shfl_xor(rw.L, 32);
+    rw.M = rw.L == 0.f ? M_LEAST : rw.M;
     const bool there = l32 < nrows;
     const int at = query * p.Hq + head;                                            // (Tq * Hq < 2^30)
     if (nsplit > 1) {
@@ -441,7 +460,7 @@ __device__ __forceinline__ void write_rows(const DeftAttn& p, const Work& w, typ
             *(t4*)(part + l32 * TL::RB + (((byte >> 4) ^ TL::fk(l32)) << 4) + (byte & 15)) = x;
         }
     DEFT_WAVE_LGKM();
-    if (p.lse && h == 0 && there) p.lse[at] = rw.L == 0.f ? -INFINITY : (rw.M + deft_log2(rw.L)) * LN2;
+    if (p.lse && h == 0 && there) p.lse[at] = log_sum(rw.M, rw.L);
 #pragma unroll
     for (int i = 0; i < TL::CPR / 2; ++i) {
         const int s = i * 64 + lane, r = s / TL::CPR, c = s - r * TL::CPR;
@@ -460,12 +479,12 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
     constexpr int NT = DT == DEFT_F32 ? 1 : 2, BN = 32 * NT, KB = BN * TL::RB, NI = BN * TL::CPR / 256;
     static_assert(NI * 256 == BN * TL::CPR, "whole DMA instructions");
     __shared__ __attribute__((aligned(1024))) char lds[4 * KB];                    // K and V of two stages (three were no faster: 124 -> 127 us, D = 64)
-    __shared__ int again;
+    __shared__ int again, far;
     const int G = p.Hq / p.Hk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     Work w;
     if (!find_work<BM>(p, TL::TS, grid, w)) return;
     const int nsplit = grid.nsplit;
-    const float sc = p.scale * LOG2E;
+    const float sc = p.scale * LOG2E, half_sc = p.scale * (LOG2E * 0.5f);
     const int left = w.rows - w.row0 - 1, wr0 = wave * 32;                         // the tile's last row, the wave's first
     const bool on = wr0 <= left;                                                   // this wave has rows
     auto query_of = [&](int r) { return w.qi + div_small(w.rem + (r < left ? r : left), grid.inv_g); };      // of row r of the tile (the last one's behind it)
@@ -487,7 +506,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
         fk.issue(w.k + (long long)t * BN * kr, base + st * 2 * KB, wave, 4, nv, kr);
         fv.issue(w.v + (long long)t * BN * vr, base + st * 2 * KB + KB, wave, 4, nv, vr);
     };
-    if (tid == 0) again = 0;
+    if (tid == 0) again = far = 0;
     if (t0 < t1) issue(t0, 0);
     typename TL::Rows rw;                                                          // (its loads and the first tile's are one trip to memory)
     rw.init((const T*)p.q + (long long)query * p.ldq + (long long)head * p.hsq, h);
@@ -499,19 +518,24 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
         const char* const ks = lds + st * 2 * KB;
         if (on && k0 < vmax) {
             const int end = k0 + BN < vend ? k0 + BN : vend;
-            if (TL::template step<NT, false>(rw, ks, ks + KB, vis - k0, vmin < k0 + BN, vmin < end, sc, lane)) again = 1;
+            const int bad = TL::template step<NT, false>(rw, ks, ks + KB, vis - k0, vmin < k0 + BN, vmin < end, sc, lane);
+            if (bad & BAD_VALUES) again = 1;
+            if (bad & FAR) far = 1;
         }
     }
+    if (rw.missed(on && t0 < t1 && vis > t0 * BN)) far = 1;
     __syncthreads();
-    if (again) {                                                                   // (rare: infinities or NaN behind the diagonal of some row)
-        rw.clear();
+    const bool half = far != 0;
+    if (again || half) {                                                           // (rare: infinities or NaN behind the diagonal of some row, far scores)
+        rw.clear(half ? M_LEAST : M_NONE);
         for (int t = t0; t < t1; ++t) {
             issue(t, 0);
             DEFT_PIPE_BARRIER(0);
-            if (on && t * BN < vmax) TL::template step<NT, true>(rw, lds, lds + KB, vis - t * BN, true, false, sc, lane);
+            if (on && t * BN < vmax) TL::template step<NT, true>(rw, lds, lds + KB, vis - t * BN, true, false, half ? half_sc : sc, lane, half);
             __syncthreads();
         }
     }
+    if (!half) rw.M *= 0.5f;
     write_rows<DT, D>(p, w, rw, nsplit, query, head, left + 1 - wr0, lane, lds + wave * KB);
 }
 
@@ -529,7 +553,7 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
     Work w;
     if (!find_work<32>(p, TL::TS, grid, w)) return;
     const int nsplit = grid.nsplit;
-    const float sc = p.scale * LOG2E;
+    const float sc = p.scale * LOG2E, half_sc = p.scale * (LOG2E * 0.5f);
     const int left = w.rows - w.row0 - 1;                                          // the tile's last row
     auto query_of = [&](int r) { return w.qi + div_small(w.rem + (r < left ? r : left), grid.inv_g); };      // of row r of the tile (the last one's behind it)
     const int rc = l32 < left ? l32 : left, qi = query_of(rc), query = w.q0 + qi, head = w.hk * G + w.rem + rc - (qi - w.qi) * G;
@@ -556,21 +580,24 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
     for (int t = t0 + wave; t < t1; t += NW, st ^= NS - 1) {
         if (NS == 2 && t + NW < t1) { DEFT_WAVE_VM(2 * NI); } else { DEFT_WAVE_VM(0); }       // this wave's tile t is here (the stages are its own: no barrier)
         const int k0 = t * 32, end = k0 + 32 < vend ? k0 + 32 : vend;
-        if (TL::template step<1, false>(rw, mine + st * 2 * KB, mine + st * 2 * KB + KB, vis - k0, vmin < k0 + 32, vmin < end, sc, lane)) again = 1;
+        again |= TL::template step<1, false>(rw, mine + st * 2 * KB, mine + st * 2 * KB + KB, vis - k0, vmin < k0 + 32, vmin < end, sc, lane);
         if (t + NS * NW < t1) {
             DEFT_WAVE_LGKM();                                                      // its reads have returned: the stage may be filled again
             issue(t + NS * NW, st);
         }
     }
-    if (again) {                                                                   // (rare: infinities or NaN behind the diagonal of some row)
-        rw.clear();
+    if (rw.missed(t0 + wave < t1 && vis > (t0 + wave) * 32)) again |= FAR;
+    const bool half = (again & FAR) != 0;
+    if (again) {                                                                   // (rare: infinities or NaN behind the diagonal of some row, far scores)
+        rw.clear(half ? M_LEAST : M_NONE);
         for (int t = t0 + wave; t < t1; t += NW) {
             DEFT_WAVE_LGKM();
             issue(t, 0);
             DEFT_WAVE_VM(0);
-            TL::template step<1, true>(rw, mine, mine + KB, vis - t * 32, true, false, sc, lane);
+            TL::template step<1, true>(rw, mine, mine + KB, vis - t * 32, true, false, half ? half_sc : sc, lane, half);
         }
     }
+    if (!half) rw.M *= 0.5f;
     if constexpr (NW == 1) {
         DEFT_WAVE_LGKM();
         write_rows<DT, D>(p, w, rw, nsplit, query, head, left + 1, lane, lds);
@@ -578,12 +605,13 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
     }
     // join the waves: everybody's M and L, then O scaled to the common M, summed in wave order
     rw.L += __shfl_xor(rw.L, 32);
+    rw.M = rw.L == 0.f ? M_LEAST : rw.M;
     if (h == 0) { ms[wave][l32] = rw.M; ls[wave][l32] = rw.L; }
     __syncthreads();
     float M = ms[0][l32];
 #pragma unroll
     for (int i = 1; i < NW; ++i) M = fmaxf(M, ms[i][l32]);
-    const float al = deft_exp2(rw.M - M);
+    const float al = deft_exp2((rw.M - M) * 2.f);
     float* const os = (float*)lds;                                                 // [wave][column][32 rows]
 #pragma unroll
     for (int j = 0; j < TL::NJ; ++j)
@@ -601,7 +629,7 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
-            Lr += ls[i][r] * deft_exp2(ms[i][r] - Mr);
+            Lr += ls[i][r] * deft_exp2((ms[i][r] - Mr) * 2.f);
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] += os[(i * D + c + e) * 32 + r];
         }
@@ -616,7 +644,7 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (T)(x[e] * inv);
             *(t4*)((T*)p.o + (long long)qr * p.ldo + (long long)hd * p.hso + c) = y;
-            if (p.lse && c == 0) p.lse[(long long)qr * p.Hq + hd] = Lr == 0.f ? -INFINITY : (Mr + deft_log2(Lr)) * LN2;
+            if (p.lse && c == 0) p.lse[(long long)qr * p.Hq + hd] = log_sum(Mr, Lr);
         }
     }
 }
@@ -630,10 +658,10 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(DeftAttn p, int nsplit)
     const int q = (int)(row / (unsigned)p.Hq), h = (int)(row - (unsigned)q * (unsigned)p.Hq);
     if (q >= p.Tq || q < p.q_start[0] || q >= p.q_start[p.B]) return;
     // lane s: M and L of split s (at most 64); then the splits' rows, whose loads wait for nothing
-    const float2 x = lane < nsplit ? *(const float2*)(ws_ml(p, nsplit) + ws_row(p, lane, q, h) * 2) : make_float2(M_NONE, 0.f);
+    const float2 x = lane < nsplit ? *(const float2*)(ws_ml(p, nsplit) + ws_row(p, lane, q, h) * 2) : make_float2(M_LEAST, 0.f);
     float M = x.x;
     for (int i = 1; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i));
-    const float al = deft_exp2(x.x - M);
+    const float al = deft_exp2((x.x - M) * 2.f);
     float L = x.y * al, o0 = 0.f, o1 = 0.f;
     for (int i = 1; i < 64; i <<= 1) L += __shfl_xor(L, i);
     const int col = lane * 2 < p.D ? lane * 2 : 0;
@@ -663,7 +691,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(DeftAttn p, int nsplit)
         const t2 y = {(T)(o0 * inv), (T)(o1 * inv)};
         *(t2*)op = y;
     }
-    if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + deft_log2(L)) * LN2;
+    if (p.lse && lane == 0) p.lse[row] = log_sum(M, L);
 }
 
 bool in_fits(long long ld, long long hs, int V) { return ld % V == 0 && hs % V == 0 && ld >= 0 && hs >= 0; }
@@ -682,7 +710,7 @@ int attn_check(const DeftAttn* d) {
                    in_fits(d->ssk, d->ssv, V) && (d->Tq <= 1 || d->ldo >= d->D) && (d->Hq <= 1 || d->hso >= d->D),
                -137, "deft_attn: strides must be multiples of %d elements and keep the rows of o apart", V);
     DEFT_CHECK(d->ldk <= (1 << 22) && d->ldv <= (1 << 22), -137, "deft_attn: ldk=%lld ldv=%lld (at most 2^22 elements between tokens)", d->ldk, d->ldv);
-    DEFT_CHECK(d->scale > 0.f && d->scale < INFINITY, -138, "deft_attn: scale=%g must be positive", (double)d->scale);
+    DEFT_CHECK(d->scale >= 0x1p-126f && d->scale <= 0x1p126f, -138, "deft_attn: scale=%g (2^-126 .. 2^126)", (double)d->scale);
     return 0;
 }
 

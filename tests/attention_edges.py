@@ -1,4 +1,6 @@
 """Corners of deft_amd.attention, shared by the CPU (SIMT emulator) and the GPU tests.  References in 64 bits and tolerances: attention_checks.py."""
+import math
+
 import torch
 
 import attention_checks as ac
@@ -75,3 +77,39 @@ def check_norm_of_far_values(lib, device, dt, size, eps):
     fine = torch.isfinite(want)
     assert torch.isfinite(got[fine]).all()
     ac.assert_rotated("far values", got[fine], want[fine], mag[fine], dt)
+
+
+def check_far_scores(lib, device, dt, size, H=2, Hk=1, D=32, nq=(3,), nk=(70,), causal=True, max_k=None, cache=None, equal=False):
+    """Finite scores of any size: the softmax of the scores as they are (`equal`: all the same, so that o is the mean of the values and lse the score plus
+    log m), never 0 or NaN because they left the range of an exponential.  Every score is exact in fp32 (few bits, one product), so it is the softmax that is
+    tested: where the scores differ, they differ by so much that the largest alone counts."""
+    g = torch.Generator().manual_seed(7)
+    b = ac.make_batch(dt, list(nq), list(nk), H, Hk, D, device, cache)
+    scale = 1.0 if abs(size) > 1e37 else 0.25                        # (q . k itself stays in fp32)
+    plan = AttentionPlan(H, Hk, D, scale=scale, device=device, lib=lib)
+    root = 2.0 ** (round(math.log2(abs(size) / scale)) // 2)
+    q = torch.zeros(b["q"].shape, dtype=torch.float64)
+    q[..., 0] = root                                                 # a score is scale * root * k[..., 0]
+    keys = []
+    for i, n in enumerate(nk):
+        k, v = (torch.zeros(n, Hk, D, dtype=torch.float64), ac.rand(g, dt, n, Hk, D))
+        k[..., 0] = size / scale / root
+        if not equal:
+            k[..., 0] *= (1 + torch.randperm(n, generator=g)[:, None] / 128)       # (8 bits: exact in every type)
+        k = k.to(dt)
+        keys.append((k, v))
+        if cache:
+            b["k"][b["slot"][i].long(), :n], b["v"][b["slot"][i].long(), :n] = k.to(device), v.to(device)
+        else:
+            at = sum(nk[:i])
+            b["k"][at:at + n], b["v"][at:at + n] = k.to(device), v.to(device)
+    q = q.to(dt).to(device)
+    kw = {n: b[n] for n in ("k_start", "slot", "k_len") if n in b}
+    o, lse = plan.attend(q, b["k"], b["v"], b["q_start"], causal=causal, max_k=max_k, lse=True, **kw)
+    for i in range(len(nq)):
+        s = slice(b["starts"][i], b["starts"][i + 1])
+        want, wl, A, mag = ac.ref_attend(q[s].cpu(), *keys[i], plan.scale, causal)
+        assert torch.isfinite(want).all() and torch.isfinite(wl).all()
+        ac.assert_attended("scores of %g, sequence %d" % (size, i), o[s], want, A, torch.zeros_like(mag), nk[i], D, dt)
+        # lse: the largest score rounded to fp32 before and after the factor 2 ln 2, and 12 u + m / 2 u of the sum
+        assert bool(((lse[s].double().cpu() - wl).abs() <= 4 * ac.U * wl.abs() + 12 * ac.U + nk[i] * ac.U / 2).all()), "lse of scores of %g" % size

@@ -25,3 +25,24 @@ def test_unturned_elements(gpu_lib, dt, adjacent, norm):
                                          (F32, 1e-30, 1e-6), (BF16, 1e19, 1e-6)])
 def test_norm_of_far_values(gpu_lib, dt, size, eps):
     ae.check_norm_of_far_values(gpu_lib, "cuda", dt, size, eps)
+
+
+FAR = [dict(size=s, equal=e) for s in (1e8, -1e8, 1e12, -1e12, 1e30, -1e30, 2e38, -2e38, -3e38, 3e38) for e in (True, False) if e or abs(s) < 1e38]
+
+
+@pytest.mark.parametrize("kw", FAR)
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_far_scores(gpu_lib, dt, kw):
+    for D in (32, 64, 96, 128):
+        ae.check_far_scores(gpu_lib, "cuda", dt, D=D, **kw)                                                    # one-wave step kernel
+        ae.check_far_scores(gpu_lib, "cuda", dt, D=D, nq=(2, 3), nk=(300, 40), max_k=300, cache="slots", **kw)     # four waves
+        ae.check_far_scores(gpu_lib, "cuda", dt, D=D, nq=(1,), nk=(600,), max_k=600, cache="slots", **kw)          # keys split
+        ae.check_far_scores(gpu_lib, "cuda", dt, D=D, nq=(80,), nk=(90,), **kw)                                # prompt kernel
+        ae.check_far_scores(gpu_lib, "cuda", dt, D=D, nq=(70,), nk=(600,), max_k=1100, causal=False, **kw)     # prompt, split
+
+
+@pytest.mark.parametrize("size", [1e5, -1e5, 1e8, -1e8])
+def test_far_scores_fp16(gpu_lib, size):
+    for equal in (True, False):
+        ae.check_far_scores(gpu_lib, "cuda", F16, size, equal=equal)
+        ae.check_far_scores(gpu_lib, "cuda", F16, size, nq=(80,), nk=(90,), equal=equal)
