@@ -8,6 +8,8 @@
 // polynomials) and keeps the 2 V values of its lane's chunks in registers for all heads it handles.
 // Measured (one MI355X, cold inputs): 32781 tokens of 32 + 8 heads of 128, bf16, norm and rotation: 145 us, 4.65 TB/s (a large copy: 5.1); 100 fp32
 // tokens of 8 + 8 heads of 32: 4.1 us on the device.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -140,9 +142,15 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
             wk[e] = p.k_weight && mine ? p.k_weight[d] : 1.f;
         }
     }
-    for (int h0 = part * slots; h0 < Hall; h0 += parts * slots) {
-        vec a2, b2;
-        load(h + parts * slots, a2, b2);
+    T* const qo = (T*)p.q_out + (long long)t * p.ldqo;
+    T* const ko = (T*)p.k_out + krow * p.ldko;
+    T* const vo = (T*)p.v_out + krow * p.ldvo;
+    const long long hsqo = p.hsqo, hsko = p.hsko, hsvo = p.hsvo;
+    // One pass's head of this lane: norm, rotation, write.  A head is far when its squares leave fp32, or the mean comes near the end of it (where the
+    // hardware's root takes no subnormal): it is brought to about 1 by a power of two first.  That is the second loop's work (in the first one its
+    // registers cost a wave a SIMD: 145 -> 155 us, 40 heads of 128): the first one ends in front of a pass with such a head (false: not written).
+    auto head = [&](auto any, int h, vec& a, vec& b) -> bool {
+        constexpr bool ANY = decltype(any)::value;
         const bool isq = h < p.Hq, isv = h >= Hqk;
         float x[V], y[V];
 #pragma unroll
@@ -154,10 +162,10 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
             ss = head_sum<LPH>(ss);
             const float m = fmaf(ss, inv_d, p.eps);
             float r = deft_rsq(m);
-            // squares that leave fp32 (or a mean near its end, where the hardware's root takes no subnormal): the head is brought to about 1 by a power
-            // of two first
             const bool far = mine && h < Hqk && !(m >= 1e-30f && ss <= 1e37f);
-            if (deft_ballot(far) != 0) {
+            if constexpr (!ANY) {
+                if (deft_ballot(far) != 0) return false;
+            } else {
                 float top = sqrtf(p.eps);
 #pragma unroll
                 for (int e = 0; e < V; ++e) top = fmaxf(top, fmaxf(fabsf(x[e]), fabsf(y[e])));
@@ -204,16 +212,29 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
 #pragma unroll
                 for (int e = 0; e < V; ++e) { a[e] = (T)x[e]; b[e] = (T)y[e]; }
             }
-            T* const dst = isq ? (T*)p.q_out + (long long)t * p.ldqo + (long long)h * p.hsqo
-                               : !isv ? (T*)p.k_out + krow * p.ldko + (long long)(h - p.Hq) * p.hsko : (T*)p.v_out + krow * p.ldvo + (long long)(h - Hqk) * p.hsvo;
+            T* const dst = isq ? qo + (long long)h * hsqo : !isv ? ko + (long long)(h - p.Hq) * hsko : vo + (long long)(h - Hqk) * hsvo;
             // (non-temporal stores write 671 MB in 139 us instead of 144.5, but the attention behind them then reads q and k from memory: 5000 fp32
             // tokens, both calls, 43 -> 57 us)
             *(vec*)(dst + lo) = a;
             *(vec*)(dst + hi) = b;
         }
+        return true;
+    };
+    int h0 = part * slots;
+    for (; h0 < Hall; h0 += parts * slots) {
+        vec a2, b2;
+        load(h + parts * slots, a2, b2);
+        if (!head(std::false_type(), h, a, b)) break;
         a = a2;
         b = b2;
         h += parts * slots;
+    }
+    if constexpr (NORM) {
+#pragma unroll 1
+        for (; h0 < Hall; h0 += parts * slots, h += parts * slots) {
+            load(h, a, b);
+            head(std::true_type(), h, a, b);
+        }
     }
 }
 

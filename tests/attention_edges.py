@@ -59,19 +59,21 @@ def check_unturned_elements(lib, device, dt, adjacent, norm):
     ac.assert_rotated("finite", got[fine], want[fine], torch.nan_to_num(mag, 0, 0, 0)[fine], dt)
 
 
-def check_norm_of_far_values(lib, device, dt, size, eps):
+def check_norm_of_far_values(lib, device, dt, size, eps, T=6, H=5, D=64, R=24, inplace=False):
     """Heads whose squares leave fp32 (above about 1e19, below about 1e-19 where eps does not hold the mean up) are normed like any other; a head of zeros
     gives zeros, one with an infinity what the formula gives: 0 beside it, NaN in its place."""
     g = torch.Generator().manual_seed(6)
-    T, H, D, R = 6, 5, 64, 24
     q = (ac.rand(g, torch.float64, T, H, D) * size).to(dt)
     q[1, 2] = 1.0                                                     # an ordinary head among them
+    if T > 6:
+        q[6:, :H - 3] = ac.rand(g, dt, T - 6, H - 3, D)                # tokens whose last heads alone are far
     if eps > 0:
         q[2, 3] = 0.0
     q[3, 1, 7] = float("inf")
     pos = torch.arange(T, dtype=torch.int32).view(T, 1)
     plan = AttentionPlan(H, 1, D, axes=(R,), eps=eps, device=device, lib=lib)
-    got = plan.norm_rotate(q.to(device), None, pos.to(device))[0].cpu()
+    x = q.to(device, copy=True)
+    got = plan.norm_rotate(x, None, pos.to(device), out=(x, None) if inplace else None)[0].cpu()
     want, mag = ac.ref_rotate(q, pos, [10000.0 ** (-i / R) for i in range(R)], [0] * R, False, norm=True, eps=eps)
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     fine = torch.isfinite(want)

@@ -27,6 +27,12 @@ def test_norm_of_far_values(gpu_lib, dt, size, eps):
     ae.check_norm_of_far_values(gpu_lib, "cuda", dt, size, eps)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_norm_of_far_values_among_others(gpu_lib, dt):
+    """Waves of several passes, a far head in the last: what the earlier passes have written in place is not read again."""
+    ae.check_norm_of_far_values(gpu_lib, "cuda", dt, 1e25, 1e-6, T=1400, H=80 if dt == F32 else 160, D=32, R=16, inplace=True)
+
+
 FAR = [dict(size=s, equal=e) for s in (1e8, -1e8, 1e12, -1e12, 1e30, -1e30, 2e38, -2e38, -3e38, 3e38) for e in (True, False) if e or abs(s) < 1e38]
 
 
