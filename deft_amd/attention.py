@@ -204,7 +204,7 @@ class AttentionPlan(_Plan):
     def attend(self, q, k, v, q_start, k_start=None, slot=None, k_len=None, causal=True, max_k=None, lse=False, out=None):
         """softmax(scale * q k^T) v of B sequences of different lengths; returns o [Tq][heads][D] (or `out`; it must not overlap k or v).
 
-        q [Tq][heads][D]; q_start [B + 1] int32 on the device: sequence b owns the query rows q_start[b] .. q_start[b + 1] - 1 (n of them).
+        q [Tq][heads][D]; q_start [B + 1] int32 on the device, growing: sequence b owns the query rows q_start[b] .. q_start[b + 1] - 1 (n of them).
         k, v [Tk][kv_heads][D]: packed; sequence b's keys are the k_len[b] rows from k_start[b] on (both default to the queries' own rows).
         k, v [slots][cap][kv_heads][D]: a cache; its keys are the k_len[b] first rows of slot slot[b].
         causal: query i of n sees the keys j <= m - n + i of its m (a lone new token sees all of them).  Rows that see no key give 0; rows of no

@@ -649,14 +649,19 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
     }
 }
 
-// Joins the splits of a row, in order: one wave a row.  Rows of no sequence have no partials and are not written.
+// Joins the splits of a row, in order: one wave a row.  Rows of no sequence have no partials and are not written; neither is any row where the starts do
+// not grow (rows between two of them may have no partials, or those of two sequences): each wave looks at all of them, 64 at a time -- few, the keys are
+// split only where there are at most about a thousand tiles.
 template <int DT>
 __global__ __launch_bounds__(256) void attn_merge_kernel(DeftAttn p, int nsplit) {
     typedef typename Elem<DT>::T T;
     const int lane = threadIdx.x & 63;
     const unsigned row = blockIdx.x * 4 + (threadIdx.x >> 6);                      // (Tq * Hq < 2^30)
     const int q = (int)(row / (unsigned)p.Hq), h = (int)(row - (unsigned)q * (unsigned)p.Hq);
-    if (q >= p.Tq || q < p.q_start[0] || q >= p.q_start[p.B]) return;
+    if (q >= p.Tq) return;
+    bool grow = true;
+    for (int b = lane; b < p.B; b += 64) grow = grow && clampi(p.q_start[b], 0, p.Tq) <= clampi(p.q_start[b + 1], 0, p.Tq);
+    if (deft_ballot(!grow || q < p.q_start[0] || q >= p.q_start[p.B]) != 0) return;
     // lane s: M and L of split s (at most 64); then the splits' rows, whose loads wait for nothing
     const float2 x = lane < nsplit ? *(const float2*)(ws_ml(p, nsplit) + ws_row(p, lane, q, h) * 2) : make_float2(M_LEAST, 0.f);
     float M = x.x;

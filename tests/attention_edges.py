@@ -115,3 +115,28 @@ def check_far_scores(lib, device, dt, size, H=2, Hk=1, D=32, nq=(3,), nk=(70,), 
         ac.assert_attended("scores of %g, sequence %d" % (size, i), o[s], want, A, torch.zeros_like(mag), nk[i], D, dt)
         # lse: the largest score rounded to fp32 before and after the factor 2 ln 2, and 12 u + m / 2 u of the sum
         assert bool(((lse[s].double().cpu() - wl).abs() <= 4 * ac.U * wl.abs() + 12 * ac.U + nk[i] * ac.U / 2).all()), "lse of scores of %g" % size
+
+
+def check_starts_that_do_not_grow(lib, device):
+    """q_start that does not grow, keys split: a row of the output is left as it was or is what one of the sequences that name it gives -- never what stood in
+    the workspace (the caller has it hold NaN)."""
+    g = torch.Generator().manual_seed(9)
+    q, k = ac.rand(g, torch.float32, 4, 2, 32).to(device), ac.rand(g, torch.float32, 900, 1, 32).to(device)
+    plan = AttentionPlan(2, 1, 32, device=device, lib=lib)
+    ks, kl = i32(device, 0, 300, 900 - 270), i32(device, 300, 280, 270)
+    for starts in ((0, 4, 2, 4), (3, 1, 0, 4), (-7, 2, 99, 3), (4, 0, 4, 0), (0, 3, 1, 4), (2, 4, 0, 2)):
+        out = torch.full((4, 2, 32), 5.0, device=device)
+        o = plan.attend(q, k, k, i32(device, *starts), k_start=ks, k_len=kl, max_k=700, out=out)
+        cut = [min(max(s, 0), 4) for s in starts]
+        for t in range(4):
+            may = [torch.full((2, 32), 5.0, dtype=torch.float64)]
+            tol = [torch.zeros(2, 32, dtype=torch.float64)]
+            for b in range(3):
+                n = cut[b + 1] - cut[b]
+                if cut[b] <= t < cut[b + 1]:
+                    a, m = int(ks[b]), int(kl[b])
+                    want, _, A, mag = ac.ref_attend(q[cut[b]:cut[b] + n].cpu(), k[a:a + m].cpu(), k[a:a + m].cpu(), plan.scale, True)
+                    may.append(want[t - cut[b]])
+                    tol.append((2 * (2 * 36 * ac.U * mag[t - cut[b]] + 8 * ac.U + m * ac.U / 2))[:, None] * A[t - cut[b]] + ac.U * want[t - cut[b]].abs())
+            got = o[t].double().cpu()
+            assert any(bool(((got - w).abs() <= e).all()) for w, e in zip(may, tol)), "starts %s, row %d" % (starts, t)

@@ -50,3 +50,9 @@ def test_far_scores_fp16(emu_lib, size):
     for equal in (True, False):
         ae.check_far_scores(emu_lib, "cpu", F16, size, equal=equal)
         ae.check_far_scores(emu_lib, "cpu", F16, size, nq=(80,), nk=(90,), equal=equal)
+
+
+def test_starts_that_do_not_grow(emu_lib, monkeypatch):
+    empty = torch.empty                                              # host memory comes back as zeros or as anything: here the workspace is NaN
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: empty(*a, **k).fill_(float("nan")) if k.get("dtype") is torch.float32 else empty(*a, **k))
+    ae.check_starts_that_do_not_grow(emu_lib, "cpu")

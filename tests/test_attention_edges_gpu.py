@@ -52,3 +52,9 @@ def test_far_scores_fp16(gpu_lib, size):
     for equal in (True, False):
         ae.check_far_scores(gpu_lib, "cuda", F16, size, equal=equal)
         ae.check_far_scores(gpu_lib, "cuda", F16, size, nq=(80,), nk=(90,), equal=equal)
+
+
+def test_starts_that_do_not_grow(gpu_lib, monkeypatch):
+    empty = torch.empty                                              # the workspace is NaN
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: empty(*a, **k).fill_(float("nan")) if k.get("dtype") is torch.float32 else empty(*a, **k))
+    ae.check_starts_that_do_not_grow(gpu_lib, "cuda")
