@@ -16,6 +16,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from .engine import _Plan
 from .hiplib import DeftHipError, _raw_stream
@@ -34,13 +35,22 @@ def _refuse(cond, *msg):
         raise DeftHipError("attention: " + msg[0] % msg[1:])
 
 
+def _no_gradient(name, x):
+    """Refuses x that needs a gradient (under torch.no_grad it needs none) or carries a forward-mode tangent: neither would come out again."""
+    if isinstance(x, torch.Tensor):
+        _refuse(x.requires_grad and torch.is_grad_enabled(), "%s requires a gradient: these operators are forward only (torch.no_grad, or detach)", name)
+        _refuse(forward_ad._current_level >= 0 and x.is_floating_point() and forward_ad.unpack_dual(x).tangent is not None,
+                "%s carries a tangent: these operators are forward only", name)
+
+
 class AttentionPlan(_Plan):
     """heads / kv_heads / head_dim of the layer (kv_heads divides heads; head h reads kv head h // (heads // kv_heads)).
 
     axes: number of rotated pairs of each position axis, e.g. (8, 12, 12) for (frame, y, x) and head_dim 64; pairs of an axis are neighbours and pair
     i turns by pos[axis] * freq[i].  freq (float64, one per pair) defaults to theta ** (-i / pairs) over all pairs; axis_of_pair overrides which
     axis a pair takes.  A pair is elements (i, i + pairs), or (2i, 2i + 1) with adjacent=True; elements behind the 2 * pairs first are not turned.
-    q_weight / k_weight [head_dim]: weights of the norms (None = 1).  scale: of the scores, 1 / sqrt(head_dim) by default."""
+    q_weight / k_weight [head_dim]: weights of the norms (None = 1).  scale: of the scores, 1 / sqrt(head_dim) by default.
+    The plan keeps copies of freq and the weights as they are when it is made."""
 
     def __init__(self, heads, kv_heads, head_dim, axes=None, theta=10000.0, freq=None, axis_of_pair=None, adjacent=False, q_weight=None, k_weight=None,
                  eps=1e-6, scale=None, device="cuda", lib=None):
@@ -58,6 +68,7 @@ class AttentionPlan(_Plan):
             self.pairs, self.naxes = sum(axes), len(axes)
             axis = [a for a, n in enumerate(axes) for _ in range(n)] if axis_of_pair is None else [int(a) for a in axis_of_pair]
             _refuse(len(axis) != self.pairs or min(axis) < 0 or max(axis) >= self.naxes, "axis_of_pair: %d values in 0 .. %d", self.pairs, self.naxes - 1)
+            _no_gradient("freq", freq)
             f = torch.tensor([theta ** (-i / self.pairs) for i in range(self.pairs)], dtype=torch.float64) if freq is None else \
                 torch.as_tensor(freq).detach().to(dtype=torch.float64, device="cpu")
             _refuse(tuple(f.shape) != (self.pairs,), "freq: one value for each of the %d pairs", self.pairs)
@@ -71,6 +82,7 @@ class AttentionPlan(_Plan):
     def _weight(self, name, w):
         if w is None:
             return None
+        _no_gradient(name, w)
         _refuse(tuple(w.shape) != (self.head_dim,), "%s has shape %s, wanted [%d]", name, tuple(w.shape), self.head_dim)
         return self.dev(w.detach().to(torch.float32).clone())
 
@@ -105,7 +117,7 @@ class AttentionPlan(_Plan):
         _refuse(x.get_device() != self._index, "%s is on %s, the plan on %s", name, x.device, self.device)
         _refuse(tokens is not None and x.shape[0] != tokens, "%s has %d tokens, wanted %s", name, x.shape[0], tokens)
         _refuse(x.stride(-1) != 1, "%s: elements of a head must be contiguous", name)
-        _refuse(torch.is_grad_enabled(), "%s requires a gradient: these operators are forward only (torch.no_grad, or detach)", name)
+        _no_gradient(name, x)
         return self._rows(name, x.detach(), heads, dtype, tokens) if lead == "[tokens]" else self._slots(name, x.detach(), dtype)
 
     def _ints(self, name, x, n):
@@ -143,9 +155,14 @@ class AttentionPlan(_Plan):
             _refuse(True, "q is %s, wanted float32, float16 or bfloat16", dt)
         ldq, hsq = self._rows("q", q, H, dt)
         T = q.shape[0]
+        if forward_ad._current_level >= 0:
+            for name, x in (("q", q), ("k", k), ("v", v), ("pos", pos), *zip(("k_cache", "v_cache"), cache or ()), *zip(("q_out", "k_out"), out or ())):
+                _no_gradient(name, x)
         pt = getattr(pos, "dtype", None)
         if not ((pt is torch.int32 or pt is torch.float32) and pos.shape == (T, self.naxes) and pos.get_device() == self._index and pos.is_contiguous()):
             _refuse(True, "pos: a contiguous int32 or float32 tensor [%d][%d] on %s", T, self.naxes, self.device)
+        if pos.requires_grad:
+            _no_gradient("pos", pos)
         q_out, k_out = out if out is not None else (None, None)
         if q_out is None:
             q_out, ldqo, hsqo = q.new_empty((T, H, D)), H * D, D
@@ -217,6 +234,9 @@ class AttentionPlan(_Plan):
             _refuse(True, "q is %s, wanted float32, float16 or bfloat16", dt)
         ldq, hsq = self._rows("q", q, H, dt)
         Tq = q.shape[0]
+        if forward_ad._current_level >= 0:
+            for name, x in (("q", q), ("k", k), ("v", v), ("out", out)):
+                _no_gradient(name, x)
         B = q_start.numel() - 1 if isinstance(q_start, torch.Tensor) else -1
         _refuse(B < 0, "q_start: B + 1 values")
         qp = self._ints("q_start", q_start, B + 1)

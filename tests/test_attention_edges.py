@@ -56,3 +56,43 @@ def test_starts_that_do_not_grow(emu_lib, monkeypatch):
     empty = torch.empty                                              # host memory comes back as zeros or as anything: here the workspace is NaN
     monkeypatch.setattr(torch, "empty", lambda *a, **k: empty(*a, **k).fill_(float("nan")) if k.get("dtype") is torch.float32 else empty(*a, **k))
     ae.check_starts_that_do_not_grow(emu_lib, "cpu")
+
+
+def test_every_gradient_is_refused(emu_lib):
+    """Weights, frequencies and positions that need a gradient, and forward-mode tangents, are refused like q, k, v: nothing drops out silently."""
+    from deft_amd.attention import AttentionPlan
+    from deft_amd.hiplib import DeftHipError
+    import torch.autograd.forward_ad as fw
+    P = lambda **kw: AttentionPlan(2, 1, 32, axes=(16,), device="cpu", lib=emu_lib, **kw)  # noqa: E731
+    w = torch.nn.Parameter(torch.ones(32))
+    f = torch.ones(16, dtype=torch.float64, requires_grad=True)
+    for kw in (dict(q_weight=w), dict(k_weight=w), dict(freq=f)):
+        with pytest.raises(DeftHipError, match="forward only"):
+            P(**kw)
+        with torch.no_grad():
+            P(**kw)
+    plan = P(q_weight=w.detach())
+    q, k, qs = torch.ones(2, 2, 32), torch.ones(2, 1, 32), torch.tensor([0, 2], dtype=torch.int32)
+    pos = torch.ones(2, 1, requires_grad=True)
+    with pytest.raises(DeftHipError, match="forward only"):
+        plan.rotate(q, k, pos)
+    with torch.no_grad():
+        plan.rotate(q, k, pos)
+    pos = pos.detach()
+    with fw.dual_level():
+        d = lambda x: fw.make_dual(x, torch.ones_like(x))  # noqa: E731
+        plan.rotate(q, k, pos), plan.attend(q, k, k, qs)                       # no tangent among them
+        for call in (lambda: plan.rotate(d(q), k, pos), lambda: plan.rotate(q, d(k), pos), lambda: plan.norm_rotate(q, k, d(pos)), lambda: plan.attend(d(q), k, k, qs),
+                     lambda: plan.attend(q, d(k), k, qs), lambda: plan.attend(q, k, d(k), qs), lambda: P(q_weight=d(torch.ones(32)))):
+            with pytest.raises(DeftHipError, match="forward only"):
+                call()
+
+
+def test_weights_are_copied(emu_lib):
+    from deft_amd.attention import AttentionPlan
+    w = torch.full((32,), 2.0)
+    plan = AttentionPlan(2, 1, 32, axes=(16,), q_weight=w, device="cpu", lib=emu_lib)
+    q, pos = torch.ones(1, 2, 32), torch.zeros(1, 1, dtype=torch.int32)
+    a = plan.norm_rotate(q, None, pos)[0]
+    w.zero_()
+    assert torch.equal(plan.norm_rotate(q, None, pos)[0], a) and a.abs().max() > 1
