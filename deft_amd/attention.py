@@ -50,12 +50,17 @@ class AttentionPlan(_Plan):
     i turns by pos[axis] * freq[i].  freq (float64, one per pair) defaults to theta ** (-i / pairs) over all pairs; axis_of_pair overrides which
     axis a pair takes.  A pair is elements (i, i + pairs), or (2i, 2i + 1) with adjacent=True; elements behind the 2 * pairs first are not turned.
     q_weight / k_weight [head_dim]: weights of the norms (None = 1).  scale: of the scores, 1 / sqrt(head_dim) by default.
+    `attend` takes head_dim 32, 64, 96 or 128; the rotations multiples of 16 (fp32: 8) up to 256, with pairs in multiples of 8 (fp32: 4).
     The plan keeps copies of freq and the weights as they are when it is made."""
 
     def __init__(self, heads, kv_heads, head_dim, axes=None, theta=10000.0, freq=None, axis_of_pair=None, adjacent=False, q_weight=None, k_weight=None,
                  eps=1e-6, scale=None, device="cuda", lib=None):
         super().__init__(device, lib)
-        _refuse(heads < 1 or kv_heads < 1 or heads % kv_heads, "heads=%d is not a multiple of kv_heads=%d", heads, kv_heads)
+        # what no call could take (types and single operators ask for more: include/deft_hip.h)
+        _refuse(heads < 1 or kv_heads < 1 or heads % kv_heads or heads > 4096, "heads=%d is not a multiple of kv_heads=%d, or above 4096", heads, kv_heads)
+        _refuse(head_dim < 8 or head_dim > 256 or head_dim % 8, "head_dim D=%d (a multiple of 8, at most 256)", head_dim)
+        _refuse(scale is not None and not 2.0 ** -126 <= scale <= 2.0 ** 126, "scale=%g (2^-126 .. 2^126)", scale)
+        _refuse(not 0.0 <= eps < math.inf, "eps=%g", eps)
         self.heads, self.kv_heads, self.head_dim = int(heads), int(kv_heads), int(head_dim)
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
         self.eps, self.adjacent = float(eps), bool(adjacent)
@@ -66,6 +71,8 @@ class AttentionPlan(_Plan):
             axes = [int(n) for n in axes]
             _refuse(not axes or min(axes) < 0 or sum(axes) < 1 or 2 * sum(axes) > head_dim, "axes=%s: 1 .. %d pairs in all", axes, head_dim // 2)
             self.pairs, self.naxes = sum(axes), len(axes)
+            _refuse(self.naxes > 8, "%d axes (at most 8)", self.naxes)
+            _refuse(self.pairs % 4, "R=%d pairs (a multiple of 4, of 8 for 16-bit types)", self.pairs)
             axis = [a for a, n in enumerate(axes) for _ in range(n)] if axis_of_pair is None else [int(a) for a in axis_of_pair]
             _refuse(len(axis) != self.pairs or min(axis) < 0 or max(axis) >= self.naxes, "axis_of_pair: %d values in 0 .. %d", self.pairs, self.naxes - 1)
             _no_gradient("freq", freq)

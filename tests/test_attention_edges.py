@@ -96,3 +96,17 @@ def test_weights_are_copied(emu_lib):
     a = plan.norm_rotate(q, None, pos)[0]
     w.zero_()
     assert torch.equal(plan.norm_rotate(q, None, pos)[0], a) and a.abs().max() > 1
+
+
+def test_plans_no_call_could_use_are_refused(emu_lib):
+    """What no call of a plan could take is refused when the plan is made; what one operator or type alone takes, at the call that does not."""
+    from deft_amd.attention import AttentionPlan
+    from deft_amd.hiplib import DeftHipError
+    P = lambda **kw: AttentionPlan(**{**dict(heads=4, kv_heads=2, head_dim=64, device="cpu", lib=emu_lib), **kw})  # noqa: E731
+    for kw, word in [(dict(axes=(13,)), "R=13 pairs"), (dict(head_dim=33), "D=33"), (dict(head_dim=0), "D=0"), (dict(head_dim=264), "D=264"), (dict(scale=0.0), "scale=0"),
+                     (dict(scale=-1.0), "scale=-1"), (dict(scale=float("nan")), "scale=nan"), (dict(scale=float("inf")), "scale=inf"), (dict(eps=-1e-6), "eps="),
+                     (dict(eps=float("nan")), "eps=nan"), (dict(heads=8192, kv_heads=8192), "4096"), (dict(axes=(4,) * 9, head_dim=128), "9 axes"), (dict(scale=1e-39), "scale=1e-39")]:
+        with pytest.raises(DeftHipError, match=word):
+            P(**kw)
+    for kw in (dict(head_dim=40, axes=(8, 12)), dict(head_dim=256, axes=(128,)), dict(axes=(4,)), dict(axes=(4,) * 8), dict(scale=2.0 ** -126), dict(eps=0.0)):
+        P(**kw)
