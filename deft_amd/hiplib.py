@@ -141,7 +141,9 @@ class HipLib:
         for name, (res, args) in _SIGS.items():
             fn = getattr(self.cdll, name + suffix, None) if suffix else None
             if fn is None:
-                fn = getattr(self.cdll, name)      # AttributeError if a symbol is not exported (host-only helpers have no twin)
+                fn = getattr(self.cdll, name, None)      # (host-only helpers have no twin)
+            if fn is None:
+                raise DeftHipError("%s does not export %s -- an older build; rebuild: python -m deft_amd.build" % (path, name))
             fn.restype = res
             fn.argtypes = args
             self._fn[name] = fn

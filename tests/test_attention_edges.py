@@ -110,3 +110,13 @@ def test_plans_no_call_could_use_are_refused(emu_lib):
             P(**kw)
     for kw in (dict(head_dim=40, axes=(8, 12)), dict(head_dim=256, axes=(128,)), dict(axes=(4,)), dict(axes=(4,) * 8), dict(scale=2.0 ** -126), dict(eps=0.0)):
         P(**kw)
+
+
+def test_an_older_library_says_rebuild(monkeypatch):
+    """A library without an entry point of this package is refused with the advice to rebuild, not with an AttributeError."""
+    import ctypes as C
+    from deft_amd import build, hiplib
+    so = build.build(force=False, verbose=False)
+    monkeypatch.setitem(hiplib._SIGS, "deft_not_yet_there", (C.c_int, []))
+    with pytest.raises(hiplib.DeftHipError, match="deft_not_yet_there.*rebuild"):
+        hiplib.HipLib(so)
