@@ -162,6 +162,8 @@ class AttentionPlan(_Plan):
             _refuse(True, "q is %s, wanted float32, float16 or bfloat16", dt)
         ldq, hsq = self._rows("q", q, H, dt)
         T = q.shape[0]
+        if T > 1 << 30:
+            _refuse(True, "q has %d tokens (at most 2^30)", T)
         if forward_ad._current_level >= 0:
             for name, x in (("q", q), ("k", k), ("v", v), ("pos", pos), *zip(("k_cache", "v_cache"), cache or ()), *zip(("q_out", "k_out"), out or ())):
                 _no_gradient(name, x)
@@ -275,9 +277,12 @@ class AttentionPlan(_Plan):
             slots, kp, vp = k.shape[0], k.data_ptr(), v.data_ptr()
             if not kp or not vp or not k.numel():               # nothing to read: every row of a sequence becomes 0
                 slots = cap = sp = lp = 0
+            if (Tq | slots | cap) >> 31:
+                _refuse(True, "Tq=%d slots=%d cap=%d", Tq, slots, cap)
             if max_k is not None:
                 longest = max(0, min(int(max_k), 0x7fffffff))
             head = (q.data_ptr(), kp, vp, out.data_ptr(), logs.data_ptr() if lse else 0, qp, sp, lp)
+            longest = min(longest, 0x7fffffff)
             tail = (ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso, ssk, ssv, Tq, B, slots, cap, H, Hk, D, _DTYPE[dt], bool(causal), longest, self.scale)
             ws, n = None, 0
             if longest > _SPLIT_KEYS:

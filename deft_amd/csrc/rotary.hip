@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
     typedef T vec __attribute__((ext_vector_type(V)));
     __shared__ __attribute__((aligned(16))) float cs_s[ROT_WAVES][2][MANY ? ROT_ANGLES : ROT_MAX_PAIRS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const unsigned unit = blockIdx.x * ROT_WAVES + wave;                           // (T * parts < 2^31)
+    const unsigned unit = blockIdx.x * ROT_WAVES + wave;                           // (at most 2^26)
     const int c = lane & (LPH - 1), sub = lane / LPH, slots = MANY ? 1 << slots_log2 : HPW;
     const int tokens = MANY ? HPW >> slots_log2 : 1, tok = MANY ? sub >> slots_log2 : 0;      // of this wave
     const int wt = __builtin_amdgcn_readfirstlane((int)(parts == 1 ? unit : unit / (unsigned)parts)), part = __builtin_amdgcn_readfirstlane((int)(unit - (unsigned)wt * (unsigned)parts));
@@ -285,7 +285,7 @@ extern "C" int deft_rotary(const DeftRotary* d, void* stream) {
                2 * ROT_MAX_PAIRS);
     DEFT_CHECK(d->R > 0 && d->R % V == 0 && 2 * d->R <= d->D, -122, "deft_rotary: R=%d pairs (a multiple of %d, 2 R <= D=%d)", d->R, V, d->D);
     DEFT_CHECK(d->A >= 1 && d->A <= 8, -122, "deft_rotary: A=%d axes (1 .. 8)", d->A);
-    DEFT_CHECK(d->T >= 0 && d->Hq > 0 && (!d->k || d->Hk > 0) && d->Hq <= 4096 && d->Hk <= 4096, -123, "deft_rotary: T=%d Hq=%d Hk=%d", d->T, d->Hq, d->Hk);
+    DEFT_CHECK(d->T >= 0 && d->T <= (1 << 30) && d->Hq > 0 && (!d->k || d->Hk > 0) && d->Hq <= 4096 && d->Hk <= 4096, -123, "deft_rotary: T=%d Hq=%d Hk=%d", d->T, d->Hq, d->Hk);
     size_t al = (size_t)d->q | (size_t)d->q_out;
     const long long orows = d->row ? d->rows : d->T;
     bool fit = in_fits(d->ldq, d->hsq, V) && out_fits(d->ldqo, d->hsqo, V, d->T, d->Hq, d->D);
@@ -316,7 +316,7 @@ extern "C" int deft_rotary(const DeftRotary* d, void* stream) {
     while ((64 / lanes) >> slots_log2 > 1) ++slots_log2;
     while (slots_log2 > 0 && heads <= 1 << (slots_log2 - 1) && d->T / (2 * tokens) >= 4096) { --slots_log2; tokens *= 2; }
     const long long units = (long long)deft_cdiv(d->T, tokens) * parts;
-    DEFT_CHECK(units < (1ll << 31), -123, "deft_rotary: T=%d", d->T);
+    DEFT_CHECK(units <= (1 << 26) - ROT_WAVES, -123, "deft_rotary: T=%d (a launch has fewer than 2^32 threads)", d->T);
     const RotLaunch l = {(unsigned)((units + ROT_WAVES - 1) / ROT_WAVES), parts, slots_log2, 1.f / (float)d->D, (hipStream_t)stream};
     if (d->dtype == DEFT_F32) rotary_launch_lanes<DEFT_F32>(*d, l, lanes);
     else if (d->dtype == DEFT_F16) rotary_launch_lanes<DEFT_F16>(*d, l, lanes);

@@ -406,7 +406,8 @@ long long deft_direct_weight_bytes(int KH, int KW, int Cin, int Cout);
  * only); k and v may be NULL, v needs k.  row != NULL: token t's k / v go to row row[t] of k_out / v_out (a cache with `rows` rows); a row
  * outside 0 .. rows-1 is not written; two tokens of one call must not name the same row.  q_out = q and (without row) k_out = k are allowed, other
  * overlaps of inputs and outputs are not.
- * One rounding to the element type at the end.  D % 16 == 0 and R % 8 == 0 (fp32: 8 and 4), D <= 256. */
+ * One rounding to the element type at the end.  D % 16 == 0 and R % 8 == 0 (fp32: 8 and 4), D <= 256, 1 .. 8 axes,
+ * T <= 2^26 - 4 (2^30 where several tokens share a wave's lanes: few heads). */
 typedef struct DeftRotary {
     const void *q, *k, *v;
     void *q_out, *k_out, *v_out;
@@ -434,7 +435,8 @@ int deft_rotary(const DeftRotary* d, void* stream);
  * and starts are DEVICE data: they are clamped to the tensors (q_start to 0 .. Tq, keys to the rows of the slot / of k), never read past them,
  * and key rows >= m are never used, whatever they hold; a masked key takes no part even where its value is an infinity or NaN.
  * max_k is a host-side estimate of the longest m that steers only how the work is split; ws / ws_floats: workspace, at least
- * deft_attn_ws_floats(d) floats (may be 0: NULL); launches that may overlap need one each.  D = 32, 64, 96 or 128. */
+ * deft_attn_ws_floats(d) floats (may be 0: NULL); launches that may overlap need one each.  D = 32, 64, 96 or 128; Tq * Hq < 2^30,
+ * B * Hk < 2^24, slots and cap <= 2^30, ldk and ldv <= 2^22, scale 2^-126 .. 2^126. */
 typedef struct DeftAttn {
     const void *q, *k, *v;
     void* o;

@@ -120,3 +120,30 @@ def test_an_older_library_says_rebuild(monkeypatch):
     monkeypatch.setitem(hiplib._SIGS, "deft_not_yet_there", (C.c_int, []))
     with pytest.raises(hiplib.DeftHipError, match="deft_not_yet_there.*rebuild"):
         hiplib.HipLib(so)
+
+
+def test_sizes_beyond_the_descriptor_are_refused(emu_lib):
+    """Token, row and slot counts past what a launch or the descriptor holds: the documented error, whatever the count (views of one token cost no memory)."""
+    import ctypes as C
+    from deft_amd.attention import AttentionPlan
+    from deft_amd.hiplib import DeftHipError, RotaryDesc
+    plan = AttentionPlan(1, 1, 32, axes=(16,), device="cpu", lib=emu_lib)
+    one = torch.zeros(1, 1, 32)
+    pos, qs, s1 = torch.zeros(1, 1, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for T in ((1 << 30) + 1, 1 << 31, 1 << 33):
+        with pytest.raises(DeftHipError, match="tokens"):
+            plan.rotate(one.expand(T, 1, 32), None, pos)
+    for n in ((1 << 30) + 1, 1 << 31, 1 << 33):
+        many = one.expand(n, 1, 32)
+        with pytest.raises(DeftHipError, match="slots="):
+            plan.attend(one, many, many, qs)
+        with pytest.raises(DeftHipError, match="cap="):
+            plan.attend(one, many[None], many[None], qs, slot=s1, k_len=s1)
+        with pytest.raises(DeftHipError, match="Tq="):
+            plan.attend(many, one, one, qs, out=torch.zeros(1, 1, 32).expand(n, 1, 32))
+    d, buf = RotaryDesc(), torch.zeros(64)
+    for f in ("q", "q_out", "pos", "freq", "axis"):
+        setattr(d, f, buf.data_ptr() + (-buf.data_ptr()) % 16)
+    d.T, d.Hq, d.Hk, d.D, d.R, d.A, d.ldq, d.hsq, d.ldqo, d.hsqo = (1 << 26) - 3, 64, 1, 8, 4, 1, 512, 8, 512, 8      # 64 heads of one lane: a wave a token
+    with pytest.raises(DeftHipError, match="T=67108861"):
+        emu_lib.call("deft_rotary", C.byref(d), None)
