@@ -8,7 +8,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRCS = [os.path.join(HERE, "csrc", f) for f in ("igemm.hip", "igemm3.hip", "dcn.hip", "direct.hip", "ops.hip", "pairmlp.hip", "rotary.hip", "attn.hip", "assoc.hip")]
-DEPS = SRCS + [os.path.join(HERE, "csrc", "common.h"), os.path.join(HERE, "..", "include", "deft_hip.h"), os.path.abspath(__file__)]
+DEPS = SRCS + [os.path.join(HERE, "csrc", "twin.cpp"), os.path.join(HERE, "csrc", "common.h"), os.path.join(HERE, "..", "include", "deft_hip.h"), os.path.abspath(__file__)]
 OUT = os.path.join(HERE, "lib", "libdeft_hip.so")
 OBJ_DIR = os.path.join(HERE, "lib", "obj")
 # dcn.hip: the SLP vectoriser turns the four-corner blend into packed fp32 math, which wants every corner weight duplicated into a
@@ -34,16 +34,19 @@ VARIANTS = {"hip": [], "bf16x3": ["-DDEFT_PIECES=3"]}
 # compiled with three bf16 pieces (no range limit: the fallback a running process switches to when an activation leaves the fp16 range,
 # deft_amd/detector.py).  The second set is the bf16x3 objects with every symbol they DEFINE renamed (llvm-objcopy --redefine-syms; references to
 # the runtime and libc are untouched; kernels are registered per object file, so equal device names in two objects do not meet).  assoc.hip is
-# host-only C++ without pieces: one copy.
+# host-only C++ without pieces: one copy.  rotary.hip and attn.hip hold device code without pieces: compiled once, their `_p3` names forward to it
+# (csrc/twin.cpp; 1.8 MB of kernels less).
 TWIN_SUFFIX = "_p3"
+NO_PIECES = ("rotary.hip", "attn.hip")
+TWIN_SRC = os.path.join(HERE, "csrc", "twin.cpp")
 OBJCOPY = "/opt/rocm/lib/llvm/bin/llvm-objcopy"
 
 
 def _twin_objects(p3_objs, verbose):
-    """Copies of the bf16x3 objects (all but assoc.hip) with every extern symbol they define renamed to <name>_p3."""
+    """Copies of the bf16x3 objects (all that depend on the pieces) with every extern symbol they define renamed to <name>_p3, and the forwarding ones."""
     twin_dir = os.path.join(HERE, "lib", "obj_twin")
     os.makedirs(twin_dir, exist_ok=True)
-    objs = [o for o in p3_objs if not o.endswith("assoc.hip.o")]
+    objs = [o for o in p3_objs if os.path.basename(o)[:-2] not in ("assoc.hip",) + NO_PIECES]
     names = set()
     for o in objs:
         for ln in subprocess.check_output(["nm", "--defined-only", "--extern-only", o], text=True).splitlines():
@@ -62,7 +65,12 @@ def _twin_objects(p3_objs, verbose):
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
         out.append(t)
-    return out
+    t = os.path.join(twin_dir, "twin.o")
+    cmd = [os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-c", TWIN_SRC, "-o", t]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return out + [t]
 
 
 def build(force=False, verbose=True, variant="hip", objects_only=False):
@@ -70,16 +78,17 @@ def build(force=False, verbose=True, variant="hip", objects_only=False):
     out = os.path.join(HERE, "lib", "libdeft_%s.so" % variant)
     obj_dir = OBJ_DIR if variant == "hip" else os.path.join(HERE, "lib", "obj_" + variant)
     os.makedirs(obj_dir, exist_ok=True)
+    os.makedirs(OBJ_DIR, exist_ok=True)
     if not force and not objects_only and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in DEPS):
         return out
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     base = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"]
     objs, jobs = [], []
     for src in SRCS:                      # one object per source: per-file flags (EXTRA), and only the edited file recompiles
-        obj = os.path.join(obj_dir, os.path.basename(src) + ".o")
+        obj = os.path.join(OBJ_DIR if os.path.basename(src) in NO_PIECES else obj_dir, os.path.basename(src) + ".o")
         objs.append(obj)
         deps = [src] + DEPS[len(SRCS):]
-        if not force and os.path.exists(obj) and all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in deps):
+        if not (force and obj.startswith(obj_dir + os.sep)) and os.path.exists(obj) and all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in deps):
             continue
         cmd = base + NO_PK_F32 + flags + EXTRA.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
         if verbose:

@@ -140,7 +140,7 @@ const char* deft_last_error(void);
 /* BOTH ARITHMETICS IN ONE LIBRARY (round 6).  Every entry point `deft_X` declared in this header whose source holds device code (everything but
  * the host-side association helpers deft_lapjv / deft_iou3d_matrix / deft_associate_* / deft_kf_*) exists a second time as `deft_X_p3` with the
  * SAME signature: the same source compiled with three bf16 pieces per operand (deft_pieces_p3() == 3; six matrix instructions per fp32 product,
- * no range limit on the activations).  Piece buffers (x3 / y3 / w3), weight images and error strings (deft_last_error_p3) belong to ONE of
+ * no range limit on the activations; the attention operators hold no pieces, their `_p3` names run the same kernels).  Piece buffers (x3 / y3 / w3), weight images and error strings (deft_last_error_p3) belong to ONE of
  * the two sets -- a caller picks per plan (all launches that exchange piece buffers from the same set).  The Python host builds its plans on
  * the `deft_X` set and moves a detector to the `_p3` set when a frame's activations leave the fp16 range (deft_amd/detector.py
  * Detector._switch_to_safe, deft_amd/hiplib.py HipLib.twin); DEFT_ARITH=bf16x3 starts there.  (Build: deft_amd/build.py links the

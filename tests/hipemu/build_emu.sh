@@ -17,13 +17,14 @@ for f in igemm igemm3 dcn direct ops pairmlp rotary attn assoc; do
     if [ ! -f $B/o2/$f.o ] || [ deft_amd/csrc/$f.hip -nt $B/o2/$f.o ] || [ deft_amd/csrc/common.h -nt $B/o2/$f.o ] || [ include/deft_hip.h -nt $B/o2/$f.o ] || [ tests/hipemu/hip/hip_runtime.h -nt $B/o2/$f.o ]; then
         X=""; [ $f = assoc ] && X="-ffp-contract=off"
         $CXX $FLAGS $X -c deft_amd/csrc/$f.hip -o $B/o2/$f.o & pids="$pids $!"
-        [ $f = assoc ] || { $CXX $FLAGS -DDEFT_PIECES=3 -c deft_amd/csrc/$f.hip -o $B/o3/$f.o & pids="$pids $!"; }
+        case $f in assoc|rotary|attn) ;; *) $CXX $FLAGS -DDEFT_PIECES=3 -c deft_amd/csrc/$f.hip -o $B/o3/$f.o & pids="$pids $!";; esac
     fi
 done
 for p in $pids; do wait $p; done
 : > $B/redefine.map
-for f in igemm igemm3 dcn direct ops pairmlp rotary attn; do nm --defined-only --extern-only $B/o3/$f.o | awk 'NF>=3 {print $NF}'; done | sort -u | awk '{print $1, $1 "_p3"}' > $B/redefine.map
+for f in igemm igemm3 dcn direct ops pairmlp; do nm --defined-only --extern-only $B/o3/$f.o | awk 'NF>=3 {print $NF}'; done | sort -u | awk '{print $1, $1 "_p3"}' > $B/redefine.map
 TW=""
-for f in igemm igemm3 dcn direct ops pairmlp rotary attn; do $OBJCOPY --redefine-syms=$B/redefine.map $B/o3/$f.o $B/o3/$f.twin.o; TW="$TW $B/o3/$f.twin.o"; done
+for f in igemm igemm3 dcn direct ops pairmlp; do $OBJCOPY --redefine-syms=$B/redefine.map $B/o3/$f.o $B/o3/$f.twin.o; TW="$TW $B/o3/$f.twin.o"; done
+$CXX -x c++ -std=c++17 -O2 -fPIC -c deft_amd/csrc/twin.cpp -o $B/o3/twin.o && TW="$TW $B/o3/twin.o"      # (rotary, attn: no pieces, deft_amd/build.py)
 $CXX -shared -pthread -o $B/libdeft_emu.so $B/o2/igemm.o $B/o2/igemm3.o $B/o2/dcn.o $B/o2/direct.o $B/o2/ops.o $B/o2/pairmlp.o $B/o2/rotary.o $B/o2/attn.o $B/o2/assoc.o $TW
 echo built tests/hipemu/_build/libdeft_emu.so

@@ -147,3 +147,27 @@ def test_sizes_beyond_the_descriptor_are_refused(emu_lib):
     d.T, d.Hq, d.Hk, d.D, d.R, d.A, d.ldq, d.hsq, d.ldqo, d.hsqo = (1 << 26) - 3, 64, 1, 8, 4, 1, 512, 8, 512, 8      # 64 heads of one lane: a wave a token
     with pytest.raises(DeftHipError, match="T=67108861"):
         emu_lib.call("deft_rotary", C.byref(d), None)
+
+
+def test_the_twins_forward(emu_lib):
+    """The `_p3` names of the operators without pieces: the same results, the refusal's text in their own set; their kernels are in the library once."""
+    import os
+    import subprocess
+    from deft_amd import build
+    from deft_amd.attention import AttentionPlan
+    from deft_amd.hiplib import DeftHipError
+    g = torch.Generator().manual_seed(0)
+    q, k, pos, qs = torch.randn(5, 2, 32, generator=g), torch.randn(5, 1, 32, generator=g), torch.arange(5, dtype=torch.int32).view(5, 1), torch.tensor([0, 5], dtype=torch.int32)
+    a, b = (AttentionPlan(2, 1, 32, axes=(16,), device="cpu", lib=x) for x in (emu_lib, emu_lib.twin()))
+    for x, y in zip(a.rotate(q, k, pos) + (a.attend(q, k, k, qs),), b.rotate(q, k, pos) + (b.attend(q, k, k, qs),)):
+        assert torch.equal(x, y)
+    p40 = AttentionPlan(2, 1, 40, device="cpu", lib=emu_lib.twin())
+    with pytest.raises(DeftHipError, match="deft_attn_p3 failed.*D=40"):
+        p40.attend(torch.zeros(5, 2, 40), torch.zeros(5, 1, 40), torch.zeros(5, 1, 40), qs)
+    with pytest.raises(DeftHipError, match="deft_attn_ws_floats_p3 failed.*D=40"):
+        p40.attend(torch.zeros(5, 2, 40), torch.zeros(5, 1, 40), torch.zeros(5, 1, 40), qs, max_k=500)
+    so = build.build(force=False, verbose=False)
+    names = subprocess.check_output(["nm", so], text=True).split()
+    for kernel in ("rotary_kernel", "attn_prompt_kernel", "attn_step_kernel", "attn_merge_kernel"):
+        stubs = [n for n in names if "__device_stub__" + kernel in n]
+        assert stubs and len(stubs) == len(set(stubs)), kernel
