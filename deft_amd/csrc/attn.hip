@@ -712,7 +712,7 @@ int attn_check(const DeftAttn* d) {
     const int V = d->dtype == DEFT_F32 ? 4 : 8;
     DEFT_CHECK((((size_t)d->q | (size_t)d->k | (size_t)d->v | (size_t)d->o) & 15) == 0, -136, "deft_attn: pointers must be 16-byte aligned");
     DEFT_CHECK(in_fits(d->ldq, d->hsq, V) && in_fits(d->ldk, d->hsk, V) && in_fits(d->ldv, d->hsv, V) && in_fits(d->ldo, d->hso, V) &&
-                   in_fits(d->ssk, d->ssv, V) && (d->Tq <= 1 || d->ldo >= d->D) && (d->Hq <= 1 || d->hso >= d->D),
+                   in_fits(d->ssk, d->ssv, V) && deft_rows_apart(d->ldo, d->hso, d->Tq, d->Hq, d->D),
                -137, "deft_attn: strides must be multiples of %d elements and keep the rows of o apart", V);
     DEFT_CHECK(d->ldk <= (1 << 22) && d->ldv <= (1 << 22), -137, "deft_attn: ldk=%lld ldv=%lld (at most 2^22 elements between tokens)", d->ldk, d->ldv);
     DEFT_CHECK(d->scale >= 0x1p-126f && d->scale <= 0x1p126f, -138, "deft_attn: scale=%g (2^-126 .. 2^126)", (double)d->scale);

@@ -249,6 +249,16 @@ __device__ __forceinline__ void deft_ws_reset(int* p) { __hip_atomic_store(p, 0,
 __device__ __forceinline__ int deft_rint(double v) { return __double2int_rn(v); }
 #endif
 
+// T x H rows of D elements, ld between tokens and hs between heads: no two share an element
+static inline bool deft_rows_apart(long long ld, long long hs, long long T, int H, int D) {
+    if ((T > 1 && ld < D) || (H > 1 && hs < D)) return false;
+    if (T <= 1 || H <= 1 || ld >= (H - 1) * hs + D || hs >= (T - 1) * ld + D) return true;
+    for (int h = 1; h < H; ++h) {                                     // (interleaved: head h of a token between the tokens on either side of h * hs)
+        const long long x = h * hs, t = x / ld;
+        if ((t < T && x - t * ld < D) || (t + 1 < T && (t + 1) * ld - x < D)) return false;
+    }
+    return true;
+}
 static inline int deft_cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // ReLU that PROPAGATES NaN (as torch.relu does; fmaxf(NaN, 0) = 0 would launder it): an operand beyond the fp16-piece range turns its

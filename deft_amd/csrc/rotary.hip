@@ -241,7 +241,7 @@ __global__ __launch_bounds__(64 * ROT_WAVES) void rotary_kernel(DeftRotary p, in
 bool in_fits(long long ld, long long hs, int V) { return ld % V == 0 && hs % V == 0 && ld >= 0 && hs >= 0; }
 // written rows must not share elements
 bool out_fits(long long ld, long long hs, int V, long long rows, int H, int D) {
-    return in_fits(ld, hs, V) && (rows <= 1 || ld >= D) && (H <= 1 || hs >= D);
+    return in_fits(ld, hs, V) && deft_rows_apart(ld, hs, rows, H, D);
 }
 
 struct RotLaunch { unsigned grid; int parts, slots_log2; float inv_d; hipStream_t s; };
@@ -298,7 +298,7 @@ extern "C" int deft_rotary(const DeftRotary* d, void* stream) {
         fit = fit && in_fits(d->ldv, d->hsv, V) && out_fits(d->ldvo, d->hsvo, V, orows, d->Hk, d->D);
     }
     DEFT_CHECK((al & 15) == 0, -124, "deft_rotary: pointers must be 16-byte aligned");
-    DEFT_CHECK(fit, -125, "deft_rotary: strides must be multiples of %d elements and keep heads apart", V);
+    DEFT_CHECK(fit, -125, "deft_rotary: strides must be multiples of %d elements and keep written rows apart", V);
     DEFT_CHECK(!d->norm || d->eps >= 0.f, -127, "deft_rotary: eps=%g", (double)d->eps);
     DEFT_CHECK(!d->row || d->rows >= 0, -126, "deft_rotary: rows=%lld", d->rows);
     if (d->T == 0) return 0;

@@ -171,3 +171,27 @@ def test_the_twins_forward(emu_lib):
     for kernel in ("rotary_kernel", "attn_prompt_kernel", "attn_step_kernel", "attn_merge_kernel"):
         stubs = [n for n in names if "__device_stub__" + kernel in n]
         assert stubs and len(stubs) == len(set(stubs)), kernel
+
+
+def test_written_rows_share_no_elements(emu_lib):
+    """Outputs and caches whose rows overlap in any way are refused; strides that only look so are taken."""
+    from deft_amd.attention import AttentionPlan
+    from deft_amd.hiplib import DeftHipError
+    g = torch.Generator().manual_seed(0)
+    plan = AttentionPlan(4, 2, 32, axes=(16,), device="cpu", lib=emu_lib)
+    q, k, pos, qs = torch.randn(4, 4, 32, generator=g), torch.randn(4, 2, 32, generator=g), torch.arange(4, dtype=torch.int32).view(4, 1), torch.tensor([0, 4], dtype=torch.int32)
+    row = torch.arange(4, dtype=torch.int32)
+    S = lambda t, h, ld, hs: torch.zeros(4096).as_strided((t, h, 32), (ld, hs, 1))  # noqa: E731
+    want, (wq, wk) = plan.attend(q, k, k, qs), plan.rotate(q, k, pos)
+    for ld, hs in ((64, 32), (32, 64), (96, 64), (160, 80), (96, 80)):                    # token 1 head 0 on token 0 head 2, ...
+        with pytest.raises(DeftHipError, match="strides"):
+            plan.attend(q, k, k, qs, out=S(4, 4, ld, hs))
+        with pytest.raises(DeftHipError, match="strides"):
+            plan.rotate(q, k, pos, out=(S(4, 4, ld, hs), None))
+    for ld, hs in ((128, 32), (32, 128), (136, 32), (288, 64), (64, 288), (32 * 7, 32 * 2), (32 * 2, 32 * 9), (160, 96)):
+        assert torch.equal(plan.attend(q, k, k, qs, out=S(4, 4, ld, hs)), want), (ld, hs)
+        assert torch.equal(plan.rotate(q, k, pos, out=(S(4, 4, ld, hs), None))[0], wq), (ld, hs)
+    with pytest.raises(DeftHipError, match="strides"):
+        plan.rotate(q, k, pos, cache=(S(8, 2, 32, 64), None), row=row)                      # row 2 of head 0 is row 0 of head 1
+    assert torch.equal(plan.rotate(q, k, pos, cache=(S(8, 2, 96, 64), None), row=row)[1][:4], wk)
+    assert torch.equal(plan.rotate(q, k, pos, cache=(S(8, 2, 96, 32), None), row=row)[1][:4], wk)
