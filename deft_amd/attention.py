@@ -85,6 +85,8 @@ class AttentionPlan(_Plan):
         self.q_weight, self.k_weight = self._weight("q_weight", q_weight), self._weight("k_weight", k_weight)
         self._qw_ptr = 0 if self.q_weight is None else self.q_weight.data_ptr()
         self._kw_ptr = 0 if self.k_weight is None else self.k_weight.data_ptr()
+        if any(w is not None and w.is_cuda for w in (q_weight, k_weight)):
+            torch.cuda.current_stream(self.device).synchronize()         # (copies from host memory have arrived; calls may come on any stream)
 
     def _weight(self, name, w):
         if w is None:

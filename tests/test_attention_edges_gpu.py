@@ -58,3 +58,27 @@ def test_starts_that_do_not_grow(gpu_lib, monkeypatch):
     empty = torch.empty                                              # the workspace is NaN
     monkeypatch.setattr(torch, "empty", lambda *a, **k: empty(*a, **k).fill_(float("nan")) if k.get("dtype") is torch.float32 else empty(*a, **k))
     ae.check_starts_that_do_not_grow(gpu_lib, "cuda")
+
+
+def test_plan_made_on_another_stream(gpu_lib):
+    """A plan's copies of its weights are there when the plan is: made on a stream that is still busy producing them, used at once on another one."""
+    from deft_amd.attention import AttentionPlan
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, pos = torch.randn(64, 4, 64, generator=g, device="cuda"), torch.arange(64, device="cuda", dtype=torch.int32).view(64, 1)
+    w = torch.rand(64, generator=g, device="cuda") + 0.5
+    want = AttentionPlan(4, 1, 64, axes=(32,), q_weight=w, device="cuda").norm_rotate(q, None, pos)[0]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    big = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(a):
+            x = big
+            for _ in range(20):
+                x = (x @ big) * 1e-2                                  # some milliseconds of work in front of the weights
+            late = w + 0.0 * x[0, :64].nan_to_num(0.0, 0.0, 0.0)
+            plan = AttentionPlan(4, 1, 64, axes=(32,), q_weight=late, device="cuda")
+        with torch.cuda.stream(b):
+            got = plan.norm_rotate(q, None, pos)[0]
+        b.synchronize()
+        assert torch.equal(got, want)
+        a.synchronize()
