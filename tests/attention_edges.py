@@ -140,3 +140,32 @@ def check_starts_that_do_not_grow(lib, device):
                     tol.append((2 * (2 * 36 * ac.U * mag[t - cut[b]] + 8 * ac.U + m * ac.U / 2))[:, None] * A[t - cut[b]] + ac.U * want[t - cut[b]].abs())
             got = o[t].double().cpu()
             assert any(bool(((got - w).abs() <= e).all()) for w, e in zip(may, tol)), "starts %s, row %d" % (starts, t)
+
+
+def check_masked_values(lib, device, dt, D, bad, nq, nk, max_k, cache="slots"):
+    """Infinities and NaN in the last keys and values of every sequence (and in all memory behind them): rows that do not see them are as close to the formula
+    as ever, rows that do come out as the formula says."""
+    def spoil(b):
+        for i, (k, v) in enumerate(b["keys"]):
+            m = k.shape[0]
+            k[-1], v[-1], v[-2, :, ::3] = bad, bad, bad
+            if cache:
+                s = int(b["slot"][i])
+                b["k"][s, :m], b["v"][s, :m] = k.to(device), v.to(device)
+            else:
+                at = sum(nk[:i])
+                b["k"][at:at + m], b["v"][at:at + m] = k.to(device), v.to(device)
+
+    b = ac.make_batch(dt, list(nq), list(nk), 2, 1, D, device, cache, seed=2, poison=bool(cache))
+    spoil(b)
+    plan = AttentionPlan(2, 1, D, device=device, lib=lib)
+    o = plan.attend(b["q"], b["k"], b["v"], b["q_start"], max_k=max_k, **{n: b[n] for n in ("k_start", "slot", "k_len") if n in b})
+    for i, (n, m) in enumerate(zip(nq, nk)):
+        got = o[b["starts"][i]:b["starts"][i + 1]]
+        want, _, A, mag = ac.ref_attend(b["queries"][i], *b["keys"][i], plan.scale, True)
+        ac.assert_attended("sequence %d, early rows" % i, got[:n - 2], want[:n - 2], A[:n - 2], mag[:n - 2], m, D, dt)
+        # the last but one sees the spoiled values of its last key (every third column); the last one sees a spoiled key
+        assert not torch.isfinite(got[n - 2, :, ::3]).any()
+        keep = [c for c in range(D) if c % 3]
+        ac.assert_attended("sequence %d, last row but one" % i, got[n - 2:n - 1, :, keep], want[n - 2:n - 1, :, keep], A[n - 2:n - 1, :, keep], mag[n - 2:n - 1], m, D, dt)
+        assert not torch.isfinite(got[n - 1]).all()

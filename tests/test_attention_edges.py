@@ -195,3 +195,23 @@ def test_written_rows_share_no_elements(emu_lib):
         plan.rotate(q, k, pos, cache=(S(8, 2, 32, 64), None), row=row)                      # row 2 of head 0 is row 0 of head 1
     assert torch.equal(plan.rotate(q, k, pos, cache=(S(8, 2, 96, 64), None), row=row)[1][:4], wk)
     assert torch.equal(plan.rotate(q, k, pos, cache=(S(8, 2, 96, 32), None), row=row)[1][:4], wk)
+
+
+MASKED = [dict(nq=(9, 3), nk=(140, 3), max_k=100),                   # step kernel, four waves
+          dict(nq=(9, 3), nk=(140, 3), max_k=700),                   # the same, keys split
+          dict(nq=(9, 3), nk=(140, 3), max_k=40),                    # one wave over long keys
+          dict(nq=(150, 4), nk=(150, 4), max_k=None, cache=None),    # prompt kernel ... (max_k None: the average is above two tiles)
+          dict(nq=(150, 4), nk=(150, 4), max_k=1100, cache=None),    # ... keys split
+          dict(nq=(200, 30), nk=(333, 30), max_k=333)]
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("late", [0, 1])
+def test_masked_values(emu_lib, dt, D, late):
+    emu_lib.cdll.hipemu_set_late_dma(late)                           # (LDS fetches delivered when issued, or when waited for)
+    try:
+        for i, kw in enumerate(MASKED):
+            ae.check_masked_values(emu_lib, "cpu", dt, D, (float("nan"), float("inf"), float("-inf"))[(i + late + D // 32) % 3], **kw)
+    finally:
+        emu_lib.cdll.hipemu_set_late_dma(0)

@@ -82,3 +82,19 @@ def test_plan_made_on_another_stream(gpu_lib):
         b.synchronize()
         assert torch.equal(got, want)
         a.synchronize()
+
+
+MASKED = [dict(nq=(9, 3), nk=(140, 3), max_k=100),                   # step kernel, four waves
+          dict(nq=(9, 3), nk=(140, 3), max_k=700),                   # the same, keys split
+          dict(nq=(9, 3), nk=(140, 3), max_k=40),                    # one wave over long keys
+          dict(nq=(150, 4), nk=(150, 4), max_k=None, cache=None),    # prompt kernel ... (max_k None: the average is above two tiles)
+          dict(nq=(150, 4), nk=(150, 4), max_k=1100, cache=None),    # ... keys split
+          dict(nq=(200, 30), nk=(333, 30), max_k=333)]
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_masked_values(gpu_lib, dt, D, bad):
+    for kw in MASKED:
+        ae.check_masked_values(gpu_lib, "cuda", dt, D, bad, **kw)
