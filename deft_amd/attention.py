@@ -239,6 +239,7 @@ class AttentionPlan(_Plan):
         sequence are not written.  Starts, lengths and slots are int32 device tensors, clamped to the tensors by the kernel; max_k (host): an
         estimate of the longest m, which steers only how the work is split (default: a cache's cap, the number of packed key rows, or the average
         length where keys are the queries' own rows).
+        Scores, statistics and sums are fp32 and o is rounded once; 16-bit prompts also round each probability to the type for its product with v.
         lse=True: returns (o, lse [Tq][heads] float32), the log of each row's sum of exponentials (-inf where it sees no key)."""
         H, Hk, D, dt = self.heads, self.kv_heads, self.head_dim, getattr(q, "dtype", None)
         if dt not in _DTYPE:

@@ -13,13 +13,18 @@
 //
 // The reference M moves only when a score exceeds it by 2^8 (P <= 2^8 then, harmless in fp32 sums and in 16-bit P): the rescaling of O and the
 // exchange between the two half-waves of a row run on few tiles instead of on all.  fp16 keeps P at 2^6 times its value, so that small
-// probabilities stay out of the subnormals.  16-bit types round each probability once for the matrix instruction (half a step relative, averaged over
-// the keys); their sum takes the unrounded ones.
+// probabilities stay out of the subnormals.
+//
+// 16-bit types round each probability for the matrix instruction; their sum takes the unrounded ones.  The step kernel gives the products the rounded part
+// AND the rest (P to 2^-16 or better; twice the products with V): its keys' bytes are the cost, and this costs little there (24 x 32000 keys: 352.8 -> 353.8
+// us, 256 x 500 64.2 -> 65.1, 2000 histories of up to 50 71.5 -> 73.4).  The prompt kernel keeps the rounded part alone, half a step relative and averaged
+// over the keys: with the rest one 16384-token sequence takes 1367 us instead of 1008, six ragged ones 172 instead of 120.  Its results are off by 1.2 to 1.4
+// times what rounding the output alone would leave.
 //
 // Two kernels:
 //   attn_prompt_kernel: 128 rows (4 waves x 32), key tiles shared by the waves, double-buffered in LDS by DMA.
-//   attn_step_kernel:   32 rows, the waves take different key tiles, each with its own double-buffered LDS, joined at the end: single tokens
-//                       over long histories, where the keys' bytes are the cost.
+//   attn_step_kernel:   32 rows, one wave or four; the waves take different key tiles, each with one or two LDS stages of its own, joined at the end: single
+//                       tokens over long histories, where the keys' bytes are the cost, and short histories.
 // Both can split the keys over workgroups (partial O, M, L in the workspace, attn_merge_kernel joins them in order).
 //
 // Measured (one MI355X, a call among others): one 16384-token sequence, 16 heads over 4 of 128, bf16, causal: 1.01 - 1.05 ms, 1050 - 1090 TFLOP/s -- MFMA busy
@@ -152,10 +157,6 @@ __device__ __forceinline__ bool find_work(const DeftAttn& p, int tsize, const Gr
     w.v = (const char*)p.v + (vo + (long long)w.hk * p.hsv) * tsize;
     return true;
 }
-// Value rows of a tile in front of this key may hold something a row must not see: rows >= m arrive as zeros (Fetch::issue), unless rows share memory
-// (a stride below a row: expanded or sliding keys) -- then the range of the source does not end with row m - 1.
-template <int D>
-__device__ __forceinline__ int values_end(const DeftAttn& p, const Work& w) { return p.ldv < D ? 0x7fffffff : w.m; }
 // keys (j < vis) that query i of the sequence sees
 __device__ __forceinline__ int visible(const DeftAttn& p, const Work& w, int i) { return p.causal ? clampi(w.m - w.n + i + 1, 0, w.m) : w.m; }
 
@@ -190,7 +191,7 @@ struct Tile {
                 off[i] = (unsigned)(r * (int)ld) * (unsigned)TS + (unsigned)c * 16u;      // (ld <= 2^22, r < 64: below 2^31)
             }
         }
-        // rows >= nv arrive as zeros: the range of the source ends with row nv - 1 (rows closer than a row: see values_end)
+        // rows >= nv arrive as zeros: the range of the source ends with row nv - 1 (where the stride is below a row they may hold the rows in front)
         __device__ __forceinline__ void issue(const char* base, lds_at lds, int first, int by, int nv, int row_bytes) const {
             const lds_src r = lds_source(base, nv <= 0 ? 0u : nv >= 64 ? 0x7FFFFFFFu : (unsigned)((nv - 1) * row_bytes + RB));
 #pragma unroll
@@ -234,29 +235,25 @@ struct Tile {
         }
         // whether some row (that saw keys: `saw`) has scores the reference could not follow down to; NaN stays NaN
         __device__ __forceinline__ bool missed(bool saw) const { return deft_ballot(saw && M == M_NONE && L == L) != 0; }
+        // whether some row's O holds an infinity or NaN that its scores do not explain: a value that is one has met a probability of 0 (a hidden key, a rest
+        // of FINE) -- or is simply seen
+        __device__ __forceinline__ bool odd() const {
+            float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z[r & 3] = fmaf(o[j][r], 0.f, z[r & 3]);
+            const float s = (z[0] + z[1]) + (z[2] + z[3]);
+            return deft_ballot(s != s && L == L) != 0;
+        }
     };
 
-    // Any infinity or NaN among the BN rows of V?
-    template <int BN>
-    static __device__ __forceinline__ bool any_bad(const char* vs, int lane) {
-        constexpr unsigned EXP = DT == DEFT_F32 ? 0x7f800000u : DT == DEFT_F16 ? 0x7c007c00u : 0x7f807f80u;
-        constexpr unsigned ONE = DT == DEFT_F32 ? 0x00800000u : DT == DEFT_F16 ? 0x04000400u : 0x00800080u;
-        unsigned bad = 0;
-#pragma unroll
-        for (int i = 0; i < BN * CPR / 64; ++i) {
-            if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);       // (16 registers at a time)
-            const u32x4 x = *(const u32x4*)(vs + (i * 64 + lane) * 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad |= (x[e] & EXP) + ONE;
-        }
-        return deft_ballot((bad & (DT == DEFT_F32 ? 0x80000000u : 0x80008000u)) != 0) != 0;
-    }
     // One tile of BN = 32 NT keys for a wave: ks, vs the tile in LDS; vis: keys of the tile this lane's row sees (may be <= 0 or > BN); `partial`
-    // (wave-uniform): some row does not see all of them; `hidden`: some row does not see keys that are there (their values must not reach it).
-    // Returns whether such hidden values are infinite or NaN (BAD_VALUES) and whether a score is beyond M_FAR (FAR): the wave's result is not valid then,
-    // and its pass is run again with CAREFUL -- with the same exponentials, or, `far`, in half log2 units (sc: scale * log2 e, or half of that).
-    template <int NT, bool CAREFUL>
-    static __device__ __forceinline__ int step(Rows& w, const char* ks, const char* vs, int vis, bool partial, bool hidden, float sc, int lane, bool far = false) {
+    // (wave-uniform): some row does not see all of them.  Returns whether a score is beyond M_FAR (FAR).  The wave's result is not valid then, nor where
+    // O is odd() at the end (BAD_VALUES): its pass is run again with CAREFUL -- with the same exponentials, or, `far`, in half log2 units (sc: scale *
+    // log2 e, or half of that).  FINE: the products take the rest of a rounded probability, too.
+    template <int NT, bool FINE, bool CAREFUL>
+    static __device__ __forceinline__ int step(Rows& w, const char* ks, const char* vs, int vis, bool partial, float sc, int lane, bool far = false) {
         const bool half = CAREFUL && far;
         const float first = half ? sc : 1.f, then = half ? 1.f : sc, units = half ? 2.f : 1.f;       // (products with 1 change nothing)
         const int h = lane >> 5;
@@ -311,18 +308,22 @@ struct Tile {
             }
         w.L += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if constexpr (CAREFUL) {
-            careful<NT>(w, s, vs, vis, lane);
+            careful<NT, FINE>(w, s, vs, vis, lane);
             return 0;
         } else {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const pfrag_t pb = probs(s[t], g);
+                    const pfrag_t p = probs(s[t], g), rest = FINE && DT != DEFT_F32 ? rest_of(s[t], g, p) : p;
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) w.o[j] = pv(value(vs, t, g, j, lane), pb, w.o[j]);
+                    for (int j = 0; j < NJ; ++j) {
+                        const pfrag_t v = value(vs, t, g, j, lane);
+                        w.o[j] = pv(v, p, w.o[j]);
+                        if constexpr (FINE && DT != DEFT_F32) w.o[j] = pv(v, rest, w.o[j]);
+                    }
                 }
-            return hidden && any_bad<32 * NT>(vs, lane) ? bad | BAD_VALUES : bad;
+            return bad;
         }
     }
 
@@ -334,6 +335,12 @@ struct Tile {
 #pragma unroll
         for (int e = 0; e < GK; ++e) p[e] = (T)s[GK * g + e];
         return p;
+    }
+    static __device__ __forceinline__ pfrag_t rest_of(const f32x16& s, int g, pfrag_t p) {
+        pfrag_t q;
+#pragma unroll
+        for (int e = 0; e < GK; ++e) q[e] = (T)(s[GK * g + e] - (float)p[e]);
+        return q;
     }
     // this lane's fragment of V^T: column 32 j + (l & 31), the keys of probs() of group g of block t
     static __device__ __forceinline__ pfrag_t value(const char* vs, int t, int g, int j, int lane) {
@@ -358,14 +365,14 @@ struct Tile {
     }
     // Products for tiles with infinities or NaN among values that not every row may see (0 * inf is NaN in a product): the finite values with P,
     // then, with P replaced by what is visible, how many +inf / NaN and how many -inf / NaN each row sees -- what is seen is added.
-    template <int NT>
+    template <int NT, bool FINE>
     static __device__ __forceinline__ void careful(Rows& w, f32x16 (&s)[NT], const char* vs, int vis, int lane) {
         const int lim = vis - 4 * (lane >> 5);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const pfrag_t p = probs(s[t], g);
+                const pfrag_t p = probs(s[t], g), rest = FINE && DT != DEFT_F32 ? rest_of(s[t], g, p) : p;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     __builtin_amdgcn_sched_barrier(0);
@@ -373,6 +380,7 @@ struct Tile {
 #pragma unroll
                     for (int e = 0; e < GK; ++e) v[e] = (float)v[e] - (float)v[e] == 0.f ? v[e] : (T)0.f;
                     w.o[j] = pv(v, p, w.o[j]);
+                    if constexpr (FINE && DT != DEFT_F32) w.o[j] = pv(v, rest, w.o[j]);
                 }
             }
 #pragma unroll
@@ -492,7 +500,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
     const int head = w.hk * G + w.rem + rc - (qi - w.qi) * G;
     const int vis = visible(p, w, qi);
     const int vmin = visible(p, w, query_of(wr0)), vmax = visible(p, w, query_of(wr0 + 31));                  // the wave's first and last row
-    const int bmax = visible(p, w, query_of(BM - 1)), vend = values_end<D>(p, w);
+    const int bmax = visible(p, w, query_of(BM - 1));
     const int nt = (bmax + BN - 1) / BN, per = split_tiles(grid, nt);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
@@ -517,21 +525,19 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(DeftAttn p, Grid gr
         const int k0 = t * BN;
         const char* const ks = lds + st * 2 * KB;
         if (on && k0 < vmax) {
-            const int end = k0 + BN < vend ? k0 + BN : vend;
-            const int bad = TL::template step<NT, false>(rw, ks, ks + KB, vis - k0, vmin < k0 + BN, vmin < end, sc, lane);
-            if (bad & BAD_VALUES) again = 1;
-            if (bad & FAR) far = 1;
+            if (TL::template step<NT, false, false>(rw, ks, ks + KB, vis - k0, vmin < k0 + BN, sc, lane)) far = 1;
         }
     }
     if (rw.missed(on && t0 < t1 && vis > t0 * BN)) far = 1;
+    if (rw.odd()) again = 1;
     __syncthreads();
     const bool half = far != 0;
-    if (again || half) {                                                           // (rare: infinities or NaN behind the diagonal of some row, far scores)
+    if (again || half) {                                                           // (rare: infinities or NaN among the values, far scores)
         rw.clear(half ? M_LEAST : M_NONE);
         for (int t = t0; t < t1; ++t) {
             issue(t, 0);
             DEFT_PIPE_BARRIER(0);
-            if (on && t * BN < vmax) TL::template step<NT, true>(rw, lds, lds + KB, vis - t * BN, true, false, half ? half_sc : sc, lane, half);
+            if (on && t * BN < vmax) TL::template step<NT, false, true>(rw, lds, lds + KB, vis - t * BN, true, half ? half_sc : sc, lane, half);
             __syncthreads();
         }
     }
@@ -557,7 +563,7 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
     const int left = w.rows - w.row0 - 1;                                          // the tile's last row
     auto query_of = [&](int r) { return w.qi + div_small(w.rem + (r < left ? r : left), grid.inv_g); };      // of row r of the tile (the last one's behind it)
     const int rc = l32 < left ? l32 : left, qi = query_of(rc), query = w.q0 + qi, head = w.hk * G + w.rem + rc - (qi - w.qi) * G;
-    const int vis = visible(p, w, qi), vmin = visible(p, w, w.qi), vmax = visible(p, w, query_of(31)), vend = values_end<D>(p, w);
+    const int vis = visible(p, w, qi), vmin = visible(p, w, w.qi), vmax = visible(p, w, query_of(31));
     const int nt = (vmax + 31) >> 5, per = split_tiles(grid, nt);
     const int t0 = w.split * per, t1 = t0 + per < nt ? t0 + per : nt;
 
@@ -579,22 +585,23 @@ __global__ __launch_bounds__(64 * NW, DT == DEFT_F32 ? (D <= 64 ? 4 : 1) : D <= 
     if (NS == 2 && t0 + wave + NW < t1) issue(t0 + wave + NW, 1);
     for (int t = t0 + wave; t < t1; t += NW, st ^= NS - 1) {
         if (NS == 2 && t + NW < t1) { DEFT_WAVE_VM(2 * NI); } else { DEFT_WAVE_VM(0); }       // this wave's tile t is here (the stages are its own: no barrier)
-        const int k0 = t * 32, end = k0 + 32 < vend ? k0 + 32 : vend;
-        again |= TL::template step<1, false>(rw, mine + st * 2 * KB, mine + st * 2 * KB + KB, vis - k0, vmin < k0 + 32, vmin < end, sc, lane);
+        const int k0 = t * 32;
+        again |= TL::template step<1, true, false>(rw, mine + st * 2 * KB, mine + st * 2 * KB + KB, vis - k0, vmin < k0 + 32, sc, lane);
         if (t + NS * NW < t1) {
             DEFT_WAVE_LGKM();                                                      // its reads have returned: the stage may be filled again
             issue(t + NS * NW, st);
         }
     }
     if (rw.missed(t0 + wave < t1 && vis > (t0 + wave) * 32)) again |= FAR;
+    if (rw.odd()) again |= BAD_VALUES;
     const bool half = (again & FAR) != 0;
-    if (again) {                                                                   // (rare: infinities or NaN behind the diagonal of some row, far scores)
+    if (again) {                                                                   // (rare: infinities or NaN among the values, far scores)
         rw.clear(half ? M_LEAST : M_NONE);
         for (int t = t0 + wave; t < t1; t += NW) {
             DEFT_WAVE_LGKM();
             issue(t, 0);
             DEFT_WAVE_VM(0);
-            TL::template step<1, true>(rw, mine, mine + KB, vis - t * 32, true, false, half ? half_sc : sc, lane, half);
+            TL::template step<1, true, true>(rw, mine, mine + KB, vis - t * 32, true, half ? half_sc : sc, lane, half);
         }
     }
     if (!half) rw.M *= 0.5f;

@@ -429,8 +429,9 @@ int deft_rotary(const DeftRotary* d, void* stream);
  *   packed (cap == 0): rows k_start[b] .. k_start[b] + m - 1 of k / v [slots][Hk][D]   (k_start NULL: q_start; k_len NULL: m = n)
  *   cache  (cap > 0):  rows 0 .. m-1 of slot k_start[b] of k / v [slots][cap][Hk][D] (slot strides ssk / ssv), m = k_len[b] -- the single-token
  *                      form: n = 1 query per track over its history
- * and query i sees key j when  !causal || j <= m - n + i.  o = softmax(scale * q k^T) v in fp32, rounded once; lse (NULL, or [Tq][Hq]
- * float) = log of the softmax's sum.  A row that sees no key, or only scores of -inf, gets o = 0 and lse = -inf.  o must not overlap k or v.  Query rows of no sequence are left as they were.  q_start
+ * and query i sees key j when  !causal || j <= m - n + i.  o = softmax(scale * q k^T) v with scores, statistics and sums in fp32, rounded
+ * once.  16-bit types: where a sequence has many queries, each probability is rounded to the type for its product with v as well (half a step relative,
+ * averaged over the keys; single tokens and short histories keep it whole).  lse (NULL, or [Tq][Hq] float) = log of the softmax's sum.  A row that sees no key, or only scores of -inf, gets o = 0 and lse = -inf.  o must not overlap k or v.  Query rows of no sequence are left as they were.  q_start
  * must grow (equal starts: no queries); where it does not, a row inside q is left as it was or holds what sequences that name it give.  Lengths
  * and starts are DEVICE data: they are clamped to the tensors (q_start to 0 .. Tq, keys to the rows of the slot / of k), never read past them,
  * and key rows >= m are never used, whatever they hold; a masked key takes no part even where its value is an infinity or NaN.

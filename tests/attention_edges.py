@@ -169,3 +169,42 @@ def check_masked_values(lib, device, dt, D, bad, nq, nk, max_k, cache="slots"):
         keep = [c for c in range(D) if c % 3]
         ac.assert_attended("sequence %d, last row but one" % i, got[n - 2:n - 1, :, keep], want[n - 2:n - 1, :, keep], A[n - 2:n - 1, :, keep], mag[n - 2:n - 1], m, D, dt)
         assert not torch.isfinite(got[n - 1]).all()
+
+
+def check_seen_infinities(lib, device, dt, D, nq, nk, max_k, cache="slots"):
+    """Infinities and NaN among the values every row sees: they come out in their columns as the formula says, whatever probability they meet; the other
+    columns are as close as ever."""
+    inf = float("inf")
+    b = ac.make_batch(dt, list(nq), list(nk), 2, 1, D, device, cache, seed=4, poison=bool(cache))
+    for i, (k, v) in enumerate(b["keys"]):
+        m = k.shape[0]
+        v[0, :, 0], v[0, :, 1], v[0, :, 2], v[1, :, 2], v[0, :, 3] = inf, -inf, inf, -inf, float("nan")
+        k[0] *= 3.0                                                    # (some rows hardly look at it)
+        if cache:
+            s = int(b["slot"][i])
+            b["k"][s, :m], b["v"][s, :m] = k.to(device), v.to(device)
+        else:
+            at = sum(nk[:i])
+            b["k"][at:at + m], b["v"][at:at + m] = k.to(device), v.to(device)
+    plan = AttentionPlan(2, 1, D, device=device, lib=lib)
+    o = plan.attend(b["q"], b["k"], b["v"], b["q_start"], max_k=max_k, causal=False, **{n: b[n] for n in ("k_start", "slot", "k_len") if n in b})
+    for i, m in enumerate(nk):
+        want, _, A, mag = ac.ref_attend(b["queries"][i], *b["keys"][i], plan.scale, False)
+        assert torch.equal(want[:, :, 0], torch.full_like(want[:, :, 0], inf)) and torch.isnan(want[:, :, 2:4]).all()
+        ac.assert_attended("sequence %d" % i, o[b["starts"][i]:b["starts"][i + 1]], want, A, mag, m, D, dt)
+
+
+def check_two_piece_steps(lib, device, dt, D, nq, nk, max_k):
+    """The step kernel's products take a probability whole (two pieces: 2^-16 relative and better): beyond the output's own rounding its error is fp32's."""
+    g = torch.Generator().manual_seed(8)
+    b = ac.make_batch(dt, list(nq), list(nk), 6, 2, D, device, "slots", seed=8)
+    plan = AttentionPlan(6, 2, D, device=device, lib=lib)
+    o = plan.attend(b["q"], b["k"], b["v"], b["q_start"], slot=b["slot"], k_len=b["k_len"], max_k=max_k)
+    for i, m in enumerate(nk):
+        want, _, A, mag = ac.ref_attend(b["queries"][i], *b["keys"][i], plan.scale, True)
+        # bf16: the rest is rounded to half a step of a number below half a step (2^-8 2^-8), fp16 likewise (2^-22) as far as its subnormals reach (2^-25 of
+        # a largest P of 2^6)
+        fine = 2.0 ** -16 if dt == torch.bfloat16 else 2.0 ** -22
+        tol = (2 * (2 * (D + 4) * ac.U * mag + 8 * ac.U + m * ac.U / 2) + fine)[..., None] * A + ac.half(dt) * want.abs() + ac.tiny(dt) + (m * 2.0 ** -31 * 8 if dt == torch.float16 else 0)
+        err = (o[b["starts"][i]:b["starts"][i + 1]].double().cpu() - want).abs()
+        assert bool((err <= tol).all()), "sequence %d: %.3g of its tolerance" % (i, float((err / tol).max()))

@@ -215,3 +215,18 @@ def test_masked_values(emu_lib, dt, D, late):
             ae.check_masked_values(emu_lib, "cpu", dt, D, (float("nan"), float("inf"), float("-inf"))[(i + late + D // 32) % 3], **kw)
     finally:
         emu_lib.cdll.hipemu_set_late_dma(0)
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_seen_infinities(emu_lib, dt, D):
+    for kw in MASKED:
+        ae.check_seen_infinities(emu_lib, "cpu", dt, D, **kw)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_step_kernels_keep_whole_probabilities(emu_lib, dt, D):
+    ae.check_two_piece_steps(emu_lib, "cpu", dt, D, (1, 1, 5), (60, 31, 5), None)             # one wave
+    ae.check_two_piece_steps(emu_lib, "cpu", dt, D, (1, 2), (900, 255), None)                 # four, keys split
+    ae.check_two_piece_steps(emu_lib, "cpu", dt, D, (1, 2), (300, 255), 200)                  # four

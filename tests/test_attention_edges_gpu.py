@@ -98,3 +98,18 @@ MASKED = [dict(nq=(9, 3), nk=(140, 3), max_k=100),                   # step kern
 def test_masked_values(gpu_lib, dt, D, bad):
     for kw in MASKED:
         ae.check_masked_values(gpu_lib, "cuda", dt, D, bad, **kw)
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_seen_infinities(gpu_lib, dt, D):
+    for kw in MASKED:
+        ae.check_seen_infinities(gpu_lib, "cuda", dt, D, **kw)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_step_kernels_keep_whole_probabilities(gpu_lib, dt, D):
+    ae.check_two_piece_steps(gpu_lib, "cuda", dt, D, (1, 1, 5), (60, 31, 5), None)             # one wave
+    ae.check_two_piece_steps(gpu_lib, "cuda", dt, D, (1, 2), (900, 255), None)                 # four, keys split
+    ae.check_two_piece_steps(gpu_lib, "cuda", dt, D, (1, 2), (300, 255), 200)                  # four
