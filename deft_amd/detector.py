@@ -14,10 +14,9 @@ from . import engine, hiplib
 
 
 import os as _os
-PRIORITY_TRACKER = _os.environ.get("DEFT_TRACKER_PRIORITY", "1") != "0"      # run(prefetch=): the tracker's launches on a high-priority stream
 # run(prefetch=): when the next frame's pass is queued -- "hook" = when the tracker announces the end of its device work (the pass then runs
 # beside the host-only rest of the association), "early" = before the tracker starts (the pass runs beside the tracker's own launches,
-# which go to the high-priority stream)
+# which go to their own stream)
 # "auto": hook for multi-frame passes (measured 2.12 vs 2.19 ms per frame at 4 frames per pass), early for one-frame passes (2.91 vs 3.18:
 # a one-frame pass queued at the hook is not finished when the next call wants it) -- tools/probe/lookahead_probe.py
 LOOKAHEAD_AT = _os.environ.get("DEFT_LOOKAHEAD_AT", "auto")
@@ -448,8 +447,9 @@ class Detector(object):
                 hook_on = last
         if nxt is not None and hook_on is None:
             nxt()
-        # a lookahead pass running (or about to be queued) beside us: the tracker's many small launches go to a HIGH-priority stream, so
-        # that they are dispatched ahead of the pass's workgroups instead of queueing behind them
+        # a lookahead pass running (or about to be queued) beside us: the tracker's many small launches go to a stream of their own instead of queueing
+        # behind it.  At the default priority, like every stream: streams of different priorities have hung, and a high one was worth nothing (one frame of
+        # lookahead 2.37 against 2.35 ms a frame, four 1.77 / 1.81 against 1.72 / 1.88)
         prio = getattr(self, "_trk_stream", None) if (self._ahead_busy() or nxt is not None) else None
         ready, self._fm_ready = getattr(self, "_fm_ready", None), None
         if prio is not None:
@@ -569,9 +569,8 @@ class Detector(object):
             if not hasattr(self, "_net_stream"):
                 self._net_stream = torch.cuda.Stream(device=self.device)
                 self._trk_done = torch.cuda.Event()
-                # the tracker's stream: never the null stream (see run()); high priority = its own hardware-queue pool, and its many
-                # small launches are dispatched ahead of the pass's workgroups
-                self._trk_stream = torch.cuda.Stream(device=self.device, priority=-1 if PRIORITY_TRACKER else 0)
+                # the tracker's stream: never the null stream (see run())
+                self._trk_stream = torch.cuda.Stream(device=self.device)
             main = torch.cuda.current_stream(self.device)
             self._trk_done.record(main)
             self._net_stream.wait_event(self._trk_done)            # whatever read this slot's feature maps (two passes ago) is finished

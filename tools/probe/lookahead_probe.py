@@ -1,4 +1,4 @@
-"""End to end with Tracker2D: serial vs one frame of lookahead (GPU).  DEFT_TRACKER_PRIORITY=0/1 python tools/probe/lookahead_probe.py"""
+"""End to end with Tracker2D: serial vs one frame of lookahead (GPU).  python tools/probe/lookahead_probe.py"""
 import os, sys, time
 import numpy as np, torch
 ROOT = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "..")

@@ -1,5 +1,5 @@
 """What makes a small launch on another stream wait for a whole lookahead pass?  (GPU)
-A 4-frame pass replayed as a hipGraph on a side stream; beside it, on stream X (null / normal / high priority): [optionally wait for an
+A 4-frame pass replayed as a hipGraph on a side stream; beside it, on stream X (null / normal): [optionally wait for an
 event recorded on the null stream] -> tiny H2D from pinned -> tiny kernel -> tiny D2H -> synchronize.  Prints the round-trip time of each
 variant while the pass is running (idle device: ~0.05 ms)."""
 import os, sys, time
@@ -30,7 +30,7 @@ print("pass alone: %.2f ms" % ((time.perf_counter() - t0) * 1e3))
 pin_in = torch.zeros(4096, dtype=torch.float32).pin_memory(); pin_out = torch.zeros(4096, dtype=torch.float32).pin_memory()
 pageable = torch.zeros(4096)
 null = torch.cuda.default_stream(dev)
-streams = {"null": null, "normal": torch.cuda.Stream(), "high": torch.cuda.Stream(priority=-1)}
+streams = {"null": null, "normal": torch.cuda.Stream()}
 
 def small(stream, wait_null, src):
     with torch.cuda.stream(stream):
