@@ -1,7 +1,7 @@
 """Attention-layer operators over tokens: detections (or map cells) at positions (frame, y, x).
 
-The second kind of sequence model next to engine.LstmPlan: where that one carries a track's history in an LSTM state row (kalman_filter_lstm.py:9-29),
-an attention layer reads the history itself.  Three operators, each one call of the C ABI (include/deft_hip.h DeftRotary, DeftAttn):
+Operators for a caller's own attention model, where engine.LstmPlan carries a track's history in an LSTM state row (kalman_filter_lstm.py:9-29) and an
+attention layer reads the history itself.  Three operators, each one call of the C ABI (include/deft_hip.h DeftRotary, DeftAttn):
 
   AttentionPlan.rotate        rotary positions with several axes on queries and keys
   AttentionPlan.norm_rotate   RMS norm of every query / key head and the rotation in one pass; keys and values into cache rows
@@ -238,7 +238,8 @@ class AttentionPlan(_Plan):
         causal: query i of n sees the keys j <= m - n + i of its m (a lone new token sees all of them).  Rows that see no key give 0; rows of no
         sequence are not written.  Starts, lengths and slots are int32 device tensors, clamped to the tensors by the kernel; max_k (host): an
         estimate of the longest m, which steers only how the work is split (default: a cache's cap, the number of packed key rows, or the average
-        length where keys are the queries' own rows).
+        length where keys are the queries' own rows).  A caller who knows better should say so: a cache with much room to grow, one long sequence among
+        short ones (up to twice the time otherwise).
         Scores, statistics and sums are fp32 and o is rounded once; 16-bit prompts also round each probability to the type for its product with v.
         lse=True: returns (o, lse [Tq][heads] float32), the log of each row's sum of exponentials (-inf where it sees no key)."""
         H, Hk, D, dt = self.heads, self.kv_heads, self.head_dim, getattr(q, "dtype", None)

@@ -27,9 +27,9 @@
 //                       tokens over long histories, where the keys' bytes are the cost, and short histories.
 // Both can split the keys over workgroups (partial O, M, L in the workspace, attn_merge_kernel joins them in order).
 //
-// Measured (one MI355X, a call among others): one 16384-token sequence, 16 heads over 4 of 128, bf16, causal: 1.01 - 1.05 ms, 1050 - 1090 TFLOP/s -- MFMA busy
+// Measured (one MI355X, a call among others): one 16384-token sequence, 16 heads over 4 of 128, bf16, causal: 1.01 - 1.07 ms, 1030 - 1090 TFLOP/s -- MFMA busy
 // 59 % and VALU 51 % of the cycles, the two of them share the clock the card holds; D = 64: 905 TFLOP/s (8 heads, 16384), VALU-bound (an exponential is
-// a quarter-rate instruction a score); 24 single tokens over 2000 .. 32000 keys, 32 heads over 8 of 128, bf16: 359 us, 5.25 TB/s of keys and values.
+// a quarter-rate instruction a score); 24 single tokens over 2000 .. 32000 keys, 32 heads over 8 of 128, bf16: 358 us, 5.25 TB/s of keys and values.
 #include "common.h"
 
 namespace {
@@ -732,7 +732,10 @@ Choice choose(const DeftAttn* d) {
     const int G = d->Hq / d->Hk;
     Choice c;
     // 32-row tiles where sequences have no more rows, or one or two key tiles (200 histories of up to 50, 4 heads a group: 12.6 us against 14.4 with
-    // 128-row tiles; 100 of 40 .. 120: 68 against 17; 4000 x 4000, D = 128: 186 against 70)
+    // 128-row tiles; 100 of 40 .. 120: 68 against 17; 4000 x 4000, D = 128: 186 against 70).  max_k is an estimate -- the AVERAGE length, where keys are the
+    // queries' own rows and the caller says nothing: one long sequence among short ones then runs on these tiles, too (8000 + 199 x 1 tokens, 16 / 4 heads
+    // of 64, bf16: 258 us against 166 on the others; 3000 + 63 x 1: 82 against 44; fp32, 8 / 8 of 32: 395 against 539).  A choice by the longest length there could be would cost the batches
+    // of short ones as much, and they are the usual ones (500 of 20 .. 64 tokens: 26.5 us against 34.7; fp32 26.2 against 47.1).
     c.step = (long long)d->Tq * G <= 32ll * d->B || d->max_k <= 64;
     const int bm = c.step ? 32 : BM;
     c.ntiles = d->Tq * G / bm + d->B;                              // (below 2^26 + 2^24)

@@ -389,7 +389,7 @@ int deft_split_weights_direct(const float* w, void* w3, int Cout, int Kpad, int 
 long long deft_direct_weight_bytes(int KH, int KW, int Cin, int Cout);
 
 /* ---- attention-layer operators over tokens (detections or map cells at positions (frame, y, x)) ---------------------------------------
- * A second kind of sequence model next to deft_lstm_step / deft_motion_step: the tokens of a track's history (or of a clip) as queries, keys
+ * For a caller's own attention model, next to deft_lstm_step / deft_motion_step: the tokens of a track's history (or of a clip) as queries, keys
  * and values.  Rows are [token][head][D] with a token stride `ld*` and a head stride `hs*` in ELEMENTS (views of one projection buffer need no
  * copy); element type `dtype`: DEFT_F32 / DEFT_F16 / DEFT_BF16, the same for all tensors of a call; every pointer to such rows is 16-byte
  * aligned and every stride a multiple of 16 bytes.  Forward only, like every entry point of this library. */
@@ -430,11 +430,12 @@ int deft_rotary(const DeftRotary* d, void* stream);
  *   cache  (cap > 0):  rows 0 .. m-1 of slot k_start[b] of k / v [slots][cap][Hk][D] (slot strides ssk / ssv), m = k_len[b] -- the single-token
  *                      form: n = 1 query per track over its history
  * and query i sees key j when  !causal || j <= m - n + i.  o = softmax(scale * q k^T) v with scores, statistics and sums in fp32, rounded
- * once.  16-bit types: where a sequence has many queries, each probability is rounded to the type for its product with v as well (half a step relative,
- * averaged over the keys; single tokens and short histories keep it whole).  lse (NULL, or [Tq][Hq] float) = log of the softmax's sum.  A row that sees no key, or only scores of -inf, gets o = 0 and lse = -inf.  o must not overlap k or v.  Query rows of no sequence are left as they were.  q_start
- * must grow (equal starts: no queries); where it does not, a row inside q is left as it was or holds what sequences that name it give.  Lengths
- * and starts are DEVICE data: they are clamped to the tensors (q_start to 0 .. Tq, keys to the rows of the slot / of k), never read past them,
- * and key rows >= m are never used, whatever they hold; a masked key takes no part even where its value is an infinity or NaN.
+ * once.  16-bit types: where a sequence has many queries, each probability is rounded to the type for its product with v as well (half a step
+ * relative, averaged over the keys; single tokens and short histories keep it whole).  lse (NULL, or [Tq][Hq] float) = log of the softmax's sum.
+ * A row that sees no key, or only scores of -inf, gets o = 0 and lse = -inf.  o must not overlap k or v.  Query rows of no sequence are left as
+ * they were.  q_start must grow (equal starts: no queries); where it does not, a row inside q is left as it was or holds what sequences that name
+ * it give.  Lengths and starts are DEVICE data: they are clamped to the tensors (q_start to 0 .. Tq, keys to the rows of the slot / of k), never
+ * read past them, and key rows >= m are never used, whatever they hold; a masked key takes no part even where its value is an infinity or NaN.
  * max_k is a host-side estimate of the longest m that steers only how the work is split; ws / ws_floats: workspace, at least
  * deft_attn_ws_floats(d) floats (may be 0: NULL); launches that may overlap need one each.  D = 32, 64, 96 or 128; Tq * Hq < 2^30,
  * B * Hk < 2^24, slots and cap <= 2^30, ldk and ldv <= 2^22, scale 2^-126 .. 2^126. */
