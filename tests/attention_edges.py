@@ -208,3 +208,63 @@ def check_two_piece_steps(lib, device, dt, D, nq, nk, max_k):
         tol = (2 * (2 * (D + 4) * ac.U * mag + 8 * ac.U + m * ac.U / 2) + fine)[..., None] * A + ac.half(dt) * want.abs() + ac.tiny(dt) + (m * 2.0 ** -31 * 8 if dt == torch.float16 else 0)
         err = (o[b["starts"][i]:b["starts"][i + 1]].double().cpu() - want).abs()
         assert bool((err <= tol).all()), "sequence %d: %.3g of its tolerance" % (i, float((err / tol).max()))
+
+
+def check_in_place(lib, device, dt):
+    """attend may write onto its queries: every kernel reads a tile's rows before it writes them."""
+    for nq, nk, max_k in (((1, 1, 5), (60, 31, 5), None), ((1, 2), (900, 255), None), ((1, 2), (300, 255), 200), ((150, 70), (150, 70), None), ((150,), (700,), 700)):
+        b = ac.make_batch(dt, list(nq), list(nk), 6, 2, 64, device, "slots", seed=11, poison=True)
+        plan = AttentionPlan(6, 2, 64, device=device, lib=lib)
+        kw = dict(slot=b["slot"], k_len=b["k_len"], max_k=max_k)
+        want = plan.attend(b["q"], b["k"], b["v"], b["q_start"], **kw)
+        got = plan.attend(b["q"], b["k"], b["v"], b["q_start"], out=b["q"], **kw)
+        assert got is b["q"] and torch.equal(got, want)
+
+
+def check_shared_keys(lib, device, dt):
+    """Sequences that read the same keys: one slot for several, windows of the packed rows that overlap."""
+    g = torch.Generator().manual_seed(12)
+    H, Hk, D = 4, 2, 32
+    plan = AttentionPlan(H, Hk, D, device=device, lib=lib)
+    nq, slots, nk = (1, 3, 1, 40), (1, 1, 0, 1), (50, 50, 7, 33)
+    qs = [0]
+    for n in nq:
+        qs.append(qs[-1] + n)
+    q, k, v = ac.rand(g, dt, qs[-1], H, D).to(device), ac.rand(g, dt, 2, 60, Hk, D).to(device), ac.rand(g, dt, 2, 60, Hk, D).to(device)
+    o = plan.attend(q, k, v, i32(device, *qs), slot=i32(device, *slots), k_len=i32(device, *nk))
+    at = (0, 20, 20, 5)
+    kp, vp = k.view(120, Hk, D), v.view(120, Hk, D)
+    op = plan.attend(q, kp, vp, i32(device, *qs), k_start=i32(device, *at), k_len=i32(device, *nk))
+    for i, n in enumerate(nq):
+        s = slice(qs[i], qs[i + 1])
+        for name, got, keys, vals in (("slot", o, k[slots[i], :nk[i]], v[slots[i], :nk[i]]), ("window", op, kp[at[i]:at[i] + nk[i]], vp[at[i]:at[i] + nk[i]])):
+            want, _, A, mag = ac.ref_attend(q[s].cpu(), keys.cpu(), vals.cpu(), plan.scale, True)
+            ac.assert_attended("%s %d" % (name, i), got[s], want, A, mag, nk[i], D, dt)
+
+
+def check_many_sequences(lib, device, dt, B):
+    """One token a sequence, thousands of them: each sees itself alone and gives its value back (P = 1 up to the fma's last step, twice rounded)."""
+    g = torch.Generator().manual_seed(13)
+    plan = AttentionPlan(2, 1, 32, device=device, lib=lib)
+    q, k, v = ac.rand(g, dt, B, 2, 32).to(device), ac.rand(g, dt, B, 1, 32).to(device), ac.rand(g, dt, B, 1, 32).to(device)
+    o, lse = plan.attend(q, k, v, torch.arange(B + 1, dtype=torch.int32, device=device), lse=True)
+    want = v.expand(B, 2, 32).double()
+    assert bool(((o.double() - want).abs() <= (ac.half(dt) + 4 * ac.U) * want.abs() + ac.tiny(dt)).all())
+    s = (q.double() * k.double()).sum(-1) * plan.scale
+    mag = (q.double() * k.double()).abs().sum(-1) * plan.scale
+    assert bool(((lse.double() - s).abs() <= 2 * 36 * ac.U * mag + 12 * ac.U).all())
+
+
+def check_far_scores_beside_masked_values(lib, device, dt, max_k):
+    """Both reasons for a second pass in one tile: scores beyond the reference's range, infinities behind the diagonal."""
+    g = torch.Generator().manual_seed(14)
+    n, D = 70, 64
+    plan = AttentionPlan(2, 1, D, scale=0.25, device=device, lib=lib)
+    q, k, v = torch.zeros(n, 2, D, dtype=torch.float64), torch.zeros(n, 1, D, dtype=torch.float64), ac.rand(g, dt, n, 1, D)
+    q[..., 0], k[..., 0] = 2.0 ** 50, -2.0 ** 50 * (1 + torch.randperm(n, generator=g)[:, None] / 128)
+    q, k = q.to(dt), k.to(dt)
+    v[-1], v[-2, :, ::3] = float("nan"), float("inf")
+    o = plan.attend(q.to(device), k.to(device), v.to(device), i32(device, 0, n), max_k=max_k)
+    want, _, A, mag = ac.ref_attend(q, k, v, plan.scale, True)
+    ac.assert_attended("rows", o[:n - 2], want[:n - 2], A[:n - 2], torch.zeros_like(mag)[:n - 2], n, D, dt)
+    assert not torch.isfinite(o[n - 1]).any() and not torch.isfinite(o[n - 2, :, ::3]).any()

@@ -230,3 +230,34 @@ def test_step_kernels_keep_whole_probabilities(emu_lib, dt, D):
     ae.check_two_piece_steps(emu_lib, "cpu", dt, D, (1, 1, 5), (60, 31, 5), None)             # one wave
     ae.check_two_piece_steps(emu_lib, "cpu", dt, D, (1, 2), (900, 255), None)                 # four, keys split
     ae.check_two_piece_steps(emu_lib, "cpu", dt, D, (1, 2), (300, 255), 200)                  # four
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+def test_attend_in_place(emu_lib, dt):
+    ae.check_in_place(emu_lib, "cpu", dt)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_sequences_that_share_keys(emu_lib, dt):
+    ae.check_shared_keys(emu_lib, "cpu", dt)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_many_sequences(emu_lib, dt):
+    ae.check_many_sequences(emu_lib, "cpu", dt, 1500)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("max_k", [40, None, 1100])
+def test_far_scores_beside_masked_values(emu_lib, dt, max_k):
+    ae.check_far_scores_beside_masked_values(emu_lib, "cpu", dt, max_k)
+
+
+@pytest.mark.parametrize("dt,D", [(F32, 8), (F32, 24), (F32, 40), (F32, 200), (F32, 256), (F16, 16), (BF16, 48), (BF16, 80), (F16, 112), (BF16, 144), (F16, 240)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rotary_widths(emu_lib, dt, D, norm):
+    """Every head width between the powers of two, more tokens than a wave holds, an odd count of heads."""
+    import attention_checks as ac
+    v = 4 if dt == F32 else 8
+    axes = (D // 2 // v * v,) if D < 4 * v else (v, D // 2 // v * v - v)
+    ac.check_rotary(emu_lib, "cpu", dt, T=37, H=5, Hk=5, D=D, axes=axes, norm=norm, adjacent=D % 32 != 0, cache="rows" if norm else None)

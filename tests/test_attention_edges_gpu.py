@@ -113,3 +113,67 @@ def test_step_kernels_keep_whole_probabilities(gpu_lib, dt, D):
     ae.check_two_piece_steps(gpu_lib, "cuda", dt, D, (1, 1, 5), (60, 31, 5), None)             # one wave
     ae.check_two_piece_steps(gpu_lib, "cuda", dt, D, (1, 2), (900, 255), None)                 # four, keys split
     ae.check_two_piece_steps(gpu_lib, "cuda", dt, D, (1, 2), (300, 255), 200)                  # four
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+def test_attend_in_place(gpu_lib, dt):
+    ae.check_in_place(gpu_lib, "cuda", dt)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_sequences_that_share_keys(gpu_lib, dt):
+    ae.check_shared_keys(gpu_lib, "cuda", dt)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_many_sequences(gpu_lib, dt):
+    ae.check_many_sequences(gpu_lib, "cuda", dt, 40000)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("max_k", [40, None, 1100])
+def test_far_scores_beside_masked_values(gpu_lib, dt, max_k):
+    ae.check_far_scores_beside_masked_values(gpu_lib, "cuda", dt, max_k)
+
+
+@pytest.mark.parametrize("dt,D", [(F32, 8), (F32, 24), (F32, 40), (F32, 200), (F32, 256), (F16, 16), (BF16, 48), (BF16, 80), (F16, 112), (BF16, 144), (F16, 240)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_rotary_widths(gpu_lib, dt, D, norm):
+    """Every head width between the powers of two, more tokens than a wave holds, an odd count of heads."""
+    import attention_checks as ac
+    v = 4 if dt == F32 else 8
+    axes = (D // 2 // v * v,) if D < 4 * v else (v, D // 2 // v * v - v)
+    ac.check_rotary(gpu_lib, "cuda", dt, T=37, H=5, Hk=5, D=D, axes=axes, norm=norm, adjacent=D % 32 != 0, cache="rows" if norm else None)
+
+
+def test_graphs_that_share_a_pool(gpu_lib):
+    """Two captured split calls whose workspaces come from one memory pool, replayed in turns with eager calls between them: the eager bits every time.  (In
+    the order of their capture, as torch asks of graphs that share a pool: the second one's output may stand where the first one's workspace was.)"""
+    from deft_amd.attention import AttentionPlan
+    g = torch.Generator(device="cuda").manual_seed(5)
+    plan = AttentionPlan(8, 2, 64, device="cuda")
+    qs, slot = torch.arange(3, device="cuda", dtype=torch.int32), torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    ln = torch.tensor([5000, 900], dtype=torch.int32, device="cuda")
+    ins = [(torch.randn(2, 8, 64, generator=g, device="cuda", dtype=BF16), torch.randn(2, 5000, 2, 64, generator=g, device="cuda", dtype=BF16)) for _ in range(2)]
+    call = lambda i: plan.attend(ins[i][0], ins[i][1], ins[i][1], qs, slot=slot, k_len=ln)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(0), call(1)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, pool = [], None
+    for i in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, pool=pool):
+            got = call(i)
+        pool = gr.pool()
+        graphs.append((gr, got))
+    for r in range(4):
+        for i in range(2):
+            ins[i][0].copy_(torch.randn(2, 8, 64, generator=g, device="cuda"))
+        want = [call(0), call(1)]
+        for gr, _ in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(graphs[i][1], want[i])
