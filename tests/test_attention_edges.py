@@ -261,3 +261,12 @@ def test_rotary_widths(emu_lib, dt, D, norm):
     v = 4 if dt == F32 else 8
     axes = (D // 2 // v * v,) if D < 4 * v else (v, D // 2 // v * v - v)
     ac.check_rotary(emu_lib, "cpu", dt, T=37, H=5, Hk=5, D=D, axes=axes, norm=norm, adjacent=D % 32 != 0, cache="rows" if norm else None)
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("known", [False, True])
+def test_one_long_sequence_among_short_ones(emu_lib, dt, known):
+    """Packed histories and one clip: by the average length (the default estimate) and by the longest one, on either kernel."""
+    import attention_checks as ac
+    n = [1, 3, 0, 2] * 10 + [260] + [1, 5] * 20
+    ac.check_attend(emu_lib, "cpu", dt, n, n, 4, 2, 64, max_k=260 if known else None)

@@ -177,3 +177,12 @@ def test_graphs_that_share_a_pool(gpu_lib):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(graphs[i][1], want[i])
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("known", [False, True])
+def test_one_long_sequence_among_short_ones(gpu_lib, dt, known):
+    """Packed histories and one clip: by the average length (the default estimate) and by the longest one, on either kernel."""
+    import attention_checks as ac
+    n = [1, 3, 0, 2] * 10 + [1500] + [1, 5] * 20
+    ac.check_attend(gpu_lib, "cuda", dt, n, n, 4, 2, 64, max_k=1500 if known else None)
